@@ -36,7 +36,7 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         return LIB
     cmd = [NVCC, *ARCH, "-O3", "-lineinfo", "-std=c++20", "-fmad=false", "--expt-relaxed-constexpr",
            "-Xcompiler", "-fPIC,-ffp-contract=off,-fvisibility=hidden", "-shared",
-           f"-I{INCLUDE}", str(CSRC / "crec.cu"), "-o", str(LIB)]
+           f"-I{INCLUDE}", "--threads", "0", *[str(s) for s in sorted(CSRC.glob("*.cu"))], "-o", str(LIB)]
     if verbose:
         cmd.insert(1, "-Xptxas=-v")
     r = subprocess.run(cmd, capture_output=True, text=True)

@@ -18,7 +18,7 @@ import numpy as np
 LIB_PATH = Path(__file__).resolve().parent / "libcarbon_rec.so"
 
 OK, E_INVALID, E_NOMEM, E_CUDA, E_STICKY, E_TIMEOUT, E_MODEL, E_RANGE = range(8)
-INT8, FP16 = 0, 1
+INT8, FP16, FP32 = 0, 1, 2
 INJECT_TIMEOUT, INJECT_STICKY = 1, 2
 _NAMES = {E_INVALID: "invalid argument", E_NOMEM: "out of memory", E_CUDA: "CUDA error", E_STICKY: "sticky CUDA error",
           E_TIMEOUT: "kernel wait timed out", E_MODEL: "model not supported", E_RANGE: "out of range"}
@@ -28,7 +28,8 @@ EXPORTS = ["crec_open", "crec_close", "crec_last_error", "crec_is_broken", "crec
            "crec_set_pages_device", "crec_recognize", "crec_recognize_lines", "crec_recognize_crops", "crec_ctc_greedy", "crec_ctc_greedy_noalloc", "crec_width_bucket", "crec_crop_region",
            "crec_stream", "crec_debug_crops", "crec_debug_value", "crec_debug_logits", "crec_last_stats", "crec_candidates",
            "crec_profile", "crec_profile_layers", "crec_mma_peak", "crec_debug_inject", "crec_conv_sweep",
-           "crec_head_sweep", "crec_ctc_head_blob"]
+           "crec_head_sweep", "crec_ctc_head_blob", "crec_logit_rules", "crec_ctc_greedy_lines", "crec_candidates_lines",
+           "crec_blob_head", "crec_adapters_open", "crec_adapters_close", "crec_adapters_logits"]
 
 
 class CrecError(RuntimeError):
@@ -81,6 +82,20 @@ class Lines(C.Structure):
                 ("frames", C.c_void_p), ("probs", C.c_void_p), ("capacity", C.c_int64), ("total", C.c_int64)]
 
 
+class LineLogits(C.Structure):
+    """The logits of packed lines on the GPU (crec_line_logits): LineLogits(logits, type, classes, pitch, rows,
+    lines, line_at), logits and line_at device addresses, type FP32 or FP16."""
+    _fields_ = [("logits", C.c_void_p), ("type", C.c_int), ("classes", C.c_int), ("pitch", C.c_int64),
+                ("rows", C.c_int64), ("lines", C.c_int), ("line_at", C.c_void_p)]
+
+
+class Rules(C.Structure):
+    """The lines' rules on the GPU (crec_rules), by keyword: device addresses, what is left out is no rule."""
+    _fields_ = [("history", C.c_void_p), ("history_at", C.c_void_p), ("repeat", C.c_void_p), ("presence", C.c_void_p),
+                ("frequency", C.c_void_p), ("bias", C.c_void_p), ("biases", C.c_int), ("bias_of", C.c_void_p),
+                ("allowed", C.c_void_p), ("sets", C.c_int), ("set_of", C.c_void_p)]
+
+
 _lib = None
 
 
@@ -121,6 +136,14 @@ def lib() -> C.CDLL:
         L.crec_conv_sweep.argtypes = [i, i, p, C.c_size_t, i, i, i, p, p, i, C.POINTER(C.c_double)]
         L.crec_head_sweep.argtypes = [i, i, p, C.c_size_t, i, p, p, p, p, i, C.POINTER(C.c_double)]
         L.crec_ctc_head_blob.argtypes = [p, C.c_size_t, p, C.c_size_t, C.POINTER(C.c_size_t), C.c_char_p, C.c_size_t]
+        z, r, e = C.POINTER(LineLogits), C.POINTER(Rules), [p, C.c_char_p, C.c_size_t]
+        L.crec_logit_rules.argtypes = [z, r, p, i, i64, *e]
+        L.crec_ctc_greedy_lines.argtypes = [z, r, p, p, p, p, *e]
+        L.crec_candidates_lines.argtypes = [z, r, i, p, p, p, *e]
+        L.crec_blob_head.argtypes = [p, C.c_size_t, C.POINTER(i), C.POINTER(i), C.c_char_p, C.c_size_t]
+        L.crec_adapters_open.argtypes = [i, p, C.c_size_t, i, p, p, p, p, C.POINTER(p), C.c_char_p, C.c_size_t]
+        L.crec_adapters_close.argtypes = [p]
+        L.crec_adapters_logits.argtypes = [p, p, i64, i64, i, p, p, p, i, i64, *e]
         _lib = L
     return _lib
 
@@ -157,6 +180,104 @@ def ctc_greedy_noalloc(logits_ptr: int, n: int, classes: int, frames: int, lengt
                                        int(ids_ptr), int(starts_ptr), int(probs_ptr), stream or None, err, 256)
     if rc != OK:
         raise CrecError(rc, err.value.decode())
+
+
+def _raise(rc: int, err) -> None:
+    raise CrecError(rc, err.value.decode())
+
+
+def logit_rules(frames: LineLogits, rules: Rules | None, out_ptr: int, out_type: int = FP32, out_pitch: int = 0,
+                stream: int = 0) -> None:
+    """crec_logit_rules: the frames' logits under their lines' rules into out (out_pitch 0: the classes);
+    queued on `stream`, not waited for."""
+    err = C.create_string_buffer(256)
+    rc = lib().crec_logit_rules(C.byref(frames), C.byref(rules) if rules is not None else None, out_ptr, out_type,
+                                out_pitch or frames.classes, stream or None, err, 256)
+    if rc != OK:
+        _raise(rc, err)
+
+
+def ctc_greedy_lines(frames: LineLogits, rules: Rules | None, counts_ptr: int, ids_ptr: int, starts_ptr: int,
+                     probs_ptr: int, stream: int = 0) -> None:
+    """crec_ctc_greedy_lines: greedy CTC of packed lines under their rules, every pointer a device address;
+    queued on `stream`, not waited for."""
+    err = C.create_string_buffer(256)
+    rc = lib().crec_ctc_greedy_lines(C.byref(frames), C.byref(rules) if rules is not None else None, counts_ptr,
+                                     ids_ptr, starts_ptr, probs_ptr, stream or None, err, 256)
+    if rc != OK:
+        _raise(rc, err)
+
+
+def candidates_lines(frames: LineLogits, rules: Rules | None, topk: int, ids_ptr: int, logp_ptr: int, blank_ptr: int,
+                     stream: int = 0) -> None:
+    """crec_candidates_lines: each frame's topk likeliest classes but the blank under its line's rules, every
+    pointer a device address; queued on `stream`, not waited for."""
+    err = C.create_string_buffer(256)
+    rc = lib().crec_candidates_lines(C.byref(frames), C.byref(rules) if rules is not None else None, topk, ids_ptr,
+                                     logp_ptr, blank_ptr, stream or None, err, 256)
+    if rc != OK:
+        _raise(rc, err)
+
+
+class Adapters:
+    """A head with low-rank adapters beside it (crec_adapters): the last 1x1 convolution of a float model
+    blob, and adapters [(A [rank, K], B [classes, rank], scale), ...], float16."""
+
+    def __init__(self, model_blob: bytes, adapters=(), device: int = 0):
+        self._h = None
+        blob = C.create_string_buffer(bytes(model_blob), len(model_blob))
+        down = [np.ascontiguousarray(a, np.float16) for a, _, _ in adapters]
+        up = [np.ascontiguousarray(b, np.float16) for _, b, _ in adapters]
+        for a, b in zip(down, up):
+            if a.ndim != 2 or b.ndim != 2 or a.shape[0] != b.shape[1]:
+                raise CrecError(E_INVALID, "an adapter is A [rank, K] and B [classes, rank]")
+        self.k, self.classes = blob_head(model_blob)
+        if any(a.shape[1] != self.k or b.shape[0] != self.classes for a, b in zip(down, up)):
+            raise CrecError(E_INVALID, f"an adapter of another head than {self.k} channels to {self.classes} classes")
+        ranks = np.array([a.shape[0] for a in down], np.int32)
+        scales = np.array([s for _, _, s in adapters], np.float32)
+        flat = [np.concatenate([m.reshape(-1) for m in ms]) if ms else np.zeros(0, np.float16) for ms in (down, up)]
+        h, err = C.c_void_p(), C.create_string_buffer(256)
+        rc = lib().crec_adapters_open(device, C.cast(blob, C.c_void_p), len(model_blob), len(down), ranks.ctypes.data,
+                                      flat[0].ctypes.data, flat[1].ctypes.data, scales.ctypes.data, C.byref(h), err, 256)
+        if rc != OK:
+            _raise(rc, err)
+        self._h = h
+
+    def logits(self, x_ptr: int, rows: int, lines: int, line_at_ptr: int, adapter_ptr: int, logits_ptr: int,
+               type: int = FP32, x_pitch: int = 0, pitch: int = 0, stream: int = 0) -> None:
+        """crec_adapters_logits: the packed lines' logits from their features, every pointer a device address
+        (pitches 0: K and the classes); queued on `stream`, not waited for."""
+        if not self._h:
+            raise CrecError(E_INVALID, "the adapters are closed")
+        err = C.create_string_buffer(256)
+        rc = lib().crec_adapters_logits(self._h, x_ptr, x_pitch or self.k, rows, lines, line_at_ptr, adapter_ptr or None,
+                                        logits_ptr, type, pitch or self.classes, stream or None, err, 256)
+        if rc != OK:
+            _raise(rc, err)
+
+    def close(self) -> None:
+        if getattr(self, "_h", None):
+            h, self._h = self._h, None
+            rc = lib().crec_adapters_close(h)
+            if rc != OK:
+                raise CrecError(rc, "crec_adapters_close")
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:  # noqa: BLE001 (interpreter shutdown: the module may be gone)
+            pass
+
+
+def blob_head(model_blob: bytes) -> tuple[int, int]:
+    """crec_blob_head: (channels K, classes) of the head of a float model blob."""
+    blob = C.create_string_buffer(bytes(model_blob), len(model_blob))
+    k, classes, err = C.c_int(0), C.c_int(0), C.create_string_buffer(256)
+    rc = lib().crec_blob_head(C.cast(blob, C.c_void_p), len(model_blob), C.byref(k), C.byref(classes), err, 256)
+    if rc != OK:
+        _raise(rc, err)
+    return k.value, classes.value
 
 
 def conv_sweep(blob: bytes, precision: int, x: np.ndarray, c_out: int, repeat: int = 3, device: int = 0,

@@ -1,0 +1,413 @@
+// The C ABI's calls on the logits of packed lines (rules, greedy CTC, candidates) and the head
+// with adapters: arguments checked, parameters filled, kernels queued.
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+#include <cstdio>
+#include <cstring>
+#include <memory>
+#include <new>
+#include <string>
+#include <vector>
+
+#include "../../include/carbon_rec.h"
+#include "adapters.cuh"
+#include "line_rules.cuh"
+
+using namespace crec;
+
+namespace {
+
+struct Errors {
+  char* text;
+  size_t size;
+  int operator()(int code, const char* msg) const {
+    if (text && size) std::snprintf(text, size, "%s", msg);
+    return code;
+  }
+  int cuda(cudaError_t e, const char* what) const {
+    char msg[256];
+    std::snprintf(msg, sizeof msg, "%s: %s", what, cudaGetErrorString(e));
+    return (*this)(e == cudaErrorMemoryAllocation ? CREC_E_NOMEM : CREC_E_CUDA, msg);
+  }
+};
+
+// The current device for a call's duration: the one that holds `array`, the caller's after it.
+class OnDeviceOf {
+ public:
+  cudaError_t enter(const void* array) {
+    cudaPointerAttributes a{};
+    cudaError_t e = cudaPointerGetAttributes(&a, array);
+    if (e != cudaSuccess) {
+      cudaGetLastError();
+      return e;
+    }
+    if (a.type != cudaMemoryTypeDevice && a.type != cudaMemoryTypeManaged) return cudaErrorInvalidDevicePointer;
+    return to(a.device);
+  }
+  cudaError_t to(int device) {
+    int cur = 0;
+    cudaError_t e = cudaGetDevice(&cur);
+    if (e != cudaSuccess || cur == device) return e;
+    if ((e = cudaSetDevice(device)) == cudaSuccess) back_ = cur;
+    return e;
+  }
+  ~OnDeviceOf() {
+    if (back_ >= 0) cudaSetDevice(back_);
+  }
+
+ private:
+  int back_ = -1;
+};
+
+size_t type_bytes(int type) { return type == CREC_FP16 ? 2 : 4; }
+bool is_logits_type(int type) { return type == CREC_FP32 || type == CREC_FP16; }
+constexpr int64_t kMaxRows = 0x7fffffff;
+constexpr int64_t kMaxPitch = int64_t{1} << 40;
+
+// What every call on packed lines checks; null where it passes.
+const char* lines_fault(const crec_line_logits* z) {
+  if (!z) return "no logits";
+  if (!is_logits_type(z->type)) return "the logits' type";
+  if (z->classes < 1) return "classes";
+  if (z->rows < 0 || z->rows > kMaxRows || z->lines < 0) return "rows or lines";
+  if (z->pitch < z->classes || z->pitch > kMaxPitch) return "pitch";
+  if (z->lines > 0 && !z->line_at) return "no line_at";
+  if (z->lines > 0 && z->rows > 0 && !z->logits) return "no logits";
+  if (reinterpret_cast<uintptr_t>(z->logits) % type_bytes(z->type)) return "the logits' alignment";
+  return nullptr;
+}
+
+const char* rules_fault(const crec_rules* r) {
+  if (!r) return nullptr;
+  if ((r->history != nullptr) != (r->history_at != nullptr)) return "history and history_at go together";
+  if (!r->history && (r->repeat || r->presence || r->frequency)) return "penalties without a history";
+  if (r->bias ? r->biases < 1 : r->bias_of != nullptr) return "bias tables";
+  if (r->allowed ? r->sets < 1 : r->set_of != nullptr) return "allowed sets";
+  return nullptr;
+}
+
+LineParams line_params(const crec_line_logits* z, const crec_rules* r) {
+  LineParams p{};
+  p.z = z->logits;
+  p.pitch = z->pitch;
+  p.classes = z->classes;
+  p.rows = static_cast<int>(z->rows);
+  p.lines = z->lines;
+  p.line_at = z->line_at;
+  p.words = static_cast<int>((static_cast<int64_t>(z->classes) + 31) / 32);
+  if (r) {
+    p.history = r->history;
+    p.history_at = r->history_at;
+    p.repeat = r->repeat;
+    p.presence = r->presence;
+    p.frequency = r->frequency;
+    p.bias = r->bias;
+    p.bias_of = r->bias_of;
+    p.biases = r->biases;
+    p.allowed = r->allowed;
+    p.set_of = r->set_of;
+    p.sets = r->sets;
+  }
+  return p;
+}
+
+template <int kOp>
+cudaError_t launch_rows(const LineParams& p, int type, cudaStream_t s) {
+  const size_t smem = p.history ? static_cast<size_t>(p.classes) * 4 : 0;
+  auto* k = type == CREC_FP16 ? line_rows_kernel<kOp, __half> : line_rows_kernel<kOp, float>;
+  if (smem > 48 << 10) {
+    const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    if (e != cudaSuccess) return e;
+  }
+  k<<<static_cast<unsigned>(p.rows), kRowThreads, smem, s>>>(p);
+  return cudaGetLastError();
+}
+
+// Whether the ruled logits may be written there: apart from the logits, exactly on them, or
+// beside them in rows of the same byte pitch.
+bool output_fits(const crec_line_logits* z, const void* out, int out_type, int64_t out_pitch) {
+  if (z->rows == 0) return true;
+  const auto a = reinterpret_cast<uintptr_t>(z->logits), b = reinterpret_cast<uintptr_t>(out);
+  const uint64_t ea = type_bytes(z->type), eb = type_bytes(out_type);
+  const uint64_t row_a = z->classes * ea, row_b = z->classes * eb, pa = z->pitch * ea, pb = out_pitch * eb;
+  const uint64_t end_a = a + (z->rows - 1) * pa + row_a, end_b = b + (z->rows - 1) * pb + row_b;
+  if (end_a <= b || end_b <= a) return true;
+  if (a == b) return z->type == out_type && (z->pitch == out_pitch || z->rows == 1);
+  if (pa != pb) return false;
+  const uint64_t d = (b > a ? (b - a) % pa : (pa - (a - b) % pa) % pa);  // out's place within the logits' rows
+  return d >= row_a && d + row_b <= pa;
+}
+
+}  // namespace
+
+struct crec_adapters {
+  int device = 0;
+  int classes = 0, k = 0, adapters = 0, rank = 0;
+  __half* w = nullptr;
+  float* bias = nullptr;
+  __half* a = nullptr;
+  __half* b = nullptr;
+  float* scale = nullptr;
+};
+
+namespace {
+
+// The last layer of a float model blob (CRECMDL1; carbon_rec/netdef.py to_blob): its weights
+// [classes][k] as float16 bits and its bias; null where it is a head, else what is wrong.
+const char* blob_head(const uint8_t* blob, size_t bytes, int* classes, int* k, std::vector<uint16_t>* w,
+                      std::vector<float>* bias) {
+  if (!blob || bytes < 40 || std::memcmp(blob, "CRECMDL1", 8) != 0) return "not a CRECMDL1 model blob";
+  uint32_t head[8];
+  std::memcpy(head, blob + 8, sizeof head);  // version, kind, values, layers, in, out, height, 0
+  if (head[0] != 1) return "model blob version";
+  if (head[1] != 1) return "a float recognizer's blob is wanted";
+  const uint64_t nv = head[2], nl = head[3];
+  if (nv > 4096 || nl > 4096 || nl == 0) return "model blob sizes";
+  uint64_t at = 40 + nv * 24;
+  for (uint64_t i = 0; i < nl; ++i) {
+    if (at + 80 > bytes) return "model blob truncated";
+    int32_t f[20];  // kind, in, out, residual, kh, kw, sh, sw, pt, pl, pb, pr, cin, cout, relu, ...
+    std::memcpy(f, blob + at, sizeof f);
+    at += 80;
+    if (f[0] == 2) {  // a Resize has no weights
+      if (i + 1 == nl) return "the last layer is no head";
+      continue;
+    }
+    if (f[4] < 1 || f[5] < 1 || f[4] > 64 || f[5] > 64 || f[12] < 1 || f[13] < 1 || f[12] > 1 << 20 || f[13] > 1 << 20 || f[19])
+      return "a layer of the model blob";
+    const uint64_t cells = static_cast<uint64_t>(f[13]) * (f[0] == 1 ? 1 : f[12]) * f[4] * f[5];
+    if (cells > bytes || at + 4 * cells + 4ull * f[13] > bytes) return "model blob truncated";
+    if (i + 1 == nl) {
+      if (f[0] != 0 || f[3] >= 0 || f[4] != 1 || f[5] != 1 || f[6] != 1 || f[7] != 1 || f[8] || f[9] || f[10] || f[11] || f[14])
+        return "the last layer is no 1x1 head";
+      *classes = f[13];
+      *k = f[12];
+      w->resize(cells);
+      for (uint64_t j = 0; j < cells; ++j) {
+        float v;
+        std::memcpy(&v, blob + at + 4 * j, 4);
+        const __half hv = __float2half_rn(v);
+        std::memcpy(&(*w)[j], &hv, 2);
+      }
+      bias->resize(f[13]);
+      std::memcpy(bias->data(), blob + at + 4 * cells, 4ull * f[13]);
+    }
+    at += 4 * cells + 4ull * f[13];
+  }
+  return at == bytes ? nullptr : "model blob has trailing bytes";
+}
+
+void free_adapters(crec_adapters* h) {
+  OnDeviceOf on;
+  if (on.to(h->device) == cudaSuccess)
+    for (void* p : {static_cast<void*>(h->w), static_cast<void*>(h->bias), static_cast<void*>(h->a),
+                    static_cast<void*>(h->b), static_cast<void*>(h->scale)})
+      cudaFree(p);
+  delete h;
+}
+
+template <class T>
+cudaError_t to_device(T** d, const void* host, size_t count) {
+  cudaError_t e = cudaMalloc(reinterpret_cast<void**>(d), std::max<size_t>(count, 1) * sizeof(T));
+  if (e == cudaSuccess && count) e = cudaMemcpy(*d, host, count * sizeof(T), cudaMemcpyHostToDevice);
+  return e;
+}
+
+int open_adapters(int device, const void* model, size_t model_bytes, int n, const int32_t* ranks, const uint16_t* a,
+                  const uint16_t* b, const float* scales, crec_adapters** out, const Errors& fail) {
+  std::vector<uint16_t> w;
+  std::vector<float> bias;
+  int classes = 0, k = 0;
+  if (const char* m = blob_head(static_cast<const uint8_t*>(model), model_bytes, &classes, &k, &w, &bias))
+    return fail(CREC_E_MODEL, m);
+  if (k % 8 || k > kMaxHeadK) return fail(CREC_E_MODEL, "adapters_open: a head of K channels, a multiple of 8, at most 512");
+  int rank = 0;
+  for (int i = 0; i < n; ++i) {
+    if (ranks[i] < 1 || ranks[i] > kMaxRank) return fail(CREC_E_RANGE, "adapters_open: a rank of 1 to 64");
+    rank = std::max(rank, static_cast<int>(ranks[i]));
+  }
+  rank = (rank + 7) / 8 * 8;
+  // A [n][rank][k] and B [n][classes][rank], the rows past an adapter's own rank 0
+  const size_t na = static_cast<size_t>(n) * rank * k, nb = static_cast<size_t>(n) * classes * rank;
+  std::vector<uint16_t> pa(na, 0), pb(nb, 0);
+  for (int i = 0; i < n; ++i) {
+    const size_t r = static_cast<size_t>(ranks[i]);
+    std::memcpy(pa.data() + static_cast<size_t>(i) * rank * k, a, r * k * 2);
+    a += r * k;
+    for (int c = 0; c < classes; ++c, b += r) std::memcpy(pb.data() + (static_cast<size_t>(i) * classes + c) * rank, b, r * 2);
+  }
+  OnDeviceOf on;
+  cudaError_t e = on.to(device);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return fail.cuda(e, "adapters_open");
+  }
+  int major = 0;
+  e = cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, device);
+  if (e == cudaSuccess && major != 10) return fail(CREC_E_INVALID, "adapters_open: this build runs on sm_100 (B200)");
+  std::unique_ptr<crec_adapters, void (*)(crec_adapters*)> h(new crec_adapters(), free_adapters);
+  h->device = device;
+  h->classes = classes;
+  h->k = k;
+  h->adapters = n;
+  h->rank = rank;
+  if (e == cudaSuccess) e = to_device(&h->w, w.data(), w.size());
+  if (e == cudaSuccess) e = to_device(&h->bias, bias.data(), bias.size());
+  if (e == cudaSuccess) e = to_device(&h->a, pa.data(), na);
+  if (e == cudaSuccess) e = to_device(&h->b, pb.data(), nb);
+  if (e == cudaSuccess) e = to_device(&h->scale, scales, static_cast<size_t>(n));
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return fail.cuda(e, "adapters_open");
+  }
+  *out = h.release();
+  return CREC_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int crec_logit_rules(const crec_line_logits* z, const crec_rules* rules, void* out, int out_type, int64_t out_pitch,
+                     void* stream, char* error, size_t error_size) {
+  const Errors fail{error, error_size};
+  if (const char* m = lines_fault(z)) return fail(CREC_E_INVALID, m);
+  if (const char* m = rules_fault(rules)) return fail(CREC_E_INVALID, m);
+  if (!is_logits_type(out_type)) return fail(CREC_E_INVALID, "logit_rules: the output's type");
+  if (out_pitch < z->classes || out_pitch > kMaxPitch) return fail(CREC_E_INVALID, "logit_rules: the output's pitch");
+  if (z->lines == 0 || z->rows == 0) return CREC_OK;
+  if (!out || reinterpret_cast<uintptr_t>(out) % type_bytes(out_type)) return fail(CREC_E_INVALID, "logit_rules: the output");
+  if (!output_fits(z, out, out_type, out_pitch)) return fail(CREC_E_INVALID, "logit_rules: the output overlaps the logits");
+  OnDeviceOf on;
+  if (const cudaError_t e = on.enter(z->logits); e != cudaSuccess) return fail.cuda(e, "logit_rules: the logits");
+  LineParams p = line_params(z, rules);
+  p.out = out;
+  p.out_half = out_type == CREC_FP16;
+  p.out_pitch = out_pitch;
+  const cudaError_t e = launch_rows<kOpRules>(p, z->type, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? CREC_OK : fail.cuda(e, "logit_rules");
+}
+
+int crec_ctc_greedy_lines(const crec_line_logits* z, const crec_rules* rules, int32_t* counts, int32_t* ids,
+                          int32_t* starts, float* probs, void* stream, char* error, size_t error_size) {
+  const Errors fail{error, error_size};
+  if (const char* m = lines_fault(z)) return fail(CREC_E_INVALID, m);
+  if (const char* m = rules_fault(rules)) return fail(CREC_E_INVALID, m);
+  if (z->lines == 0) return CREC_OK;
+  if (!counts || (z->rows > 0 && (!ids || !starts || !probs))) return fail(CREC_E_INVALID, "ctc_greedy_lines: no output");
+  OnDeviceOf on;
+  if (const cudaError_t e = on.enter(counts); e != cudaSuccess) return fail.cuda(e, "ctc_greedy_lines: counts");
+  LineParams p = line_params(z, rules);
+  p.counts = counts;
+  p.ids = ids;
+  p.starts = starts;
+  p.probs = probs;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  cudaError_t e = p.rows > 0 ? launch_rows<kOpGreedy>(p, z->type, s) : cudaSuccess;
+  if (e == cudaSuccess) {
+    collapse_lines_kernel<<<(p.lines + 3) / 4, 128, 0, s>>>(p);
+    e = cudaGetLastError();
+  }
+  return e == cudaSuccess ? CREC_OK : fail.cuda(e, "ctc_greedy_lines");
+}
+
+int crec_candidates_lines(const crec_line_logits* z, const crec_rules* rules, int topk, int32_t* ids, float* logp,
+                          float* blank, void* stream, char* error, size_t error_size) {
+  const Errors fail{error, error_size};
+  if (const char* m = lines_fault(z)) return fail(CREC_E_INVALID, m);
+  if (const char* m = rules_fault(rules)) return fail(CREC_E_INVALID, m);
+  if (topk < 0 || topk > std::min(16, z->classes - 1))
+    return fail(CREC_E_RANGE, "candidates_lines: topk is 0 to min(16, classes - 1)");
+  if (z->lines == 0 || z->rows == 0) return CREC_OK;
+  if (!blank || (topk > 0 && (!ids || !logp))) return fail(CREC_E_INVALID, "candidates_lines: no output");
+  OnDeviceOf on;
+  if (const cudaError_t e = on.enter(z->logits); e != cudaSuccess) return fail.cuda(e, "candidates_lines: the logits");
+  LineParams p = line_params(z, rules);
+  p.ids = ids;
+  p.probs = logp;
+  p.blank = blank;
+  p.topk = topk;
+  const cudaError_t e = launch_rows<kOpCandidates>(p, z->type, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? CREC_OK : fail.cuda(e, "candidates_lines");
+}
+
+int crec_blob_head(const void* model, size_t model_bytes, int* k, int* classes, char* error, size_t error_size) {
+  const Errors fail{error, error_size};
+  if (!k || !classes) return fail(CREC_E_INVALID, "blob_head: arguments");
+  try {
+    std::vector<uint16_t> w;
+    std::vector<float> bias;
+    const char* m = blob_head(static_cast<const uint8_t*>(model), model_bytes, classes, k, &w, &bias);
+    return m ? fail(CREC_E_MODEL, m) : CREC_OK;
+  } catch (const std::bad_alloc&) {
+    return fail(CREC_E_NOMEM, "blob_head: host memory");
+  }
+}
+
+int crec_adapters_open(int device, const void* model, size_t model_bytes, int n, const int32_t* ranks, const void* a,
+                       const void* b, const float* scales, crec_adapters** out, char* error, size_t error_size) {
+  const Errors fail{error, error_size};
+  if (!out) return fail(CREC_E_INVALID, "adapters_open: no handle to fill");
+  *out = nullptr;
+  if (device < 0 || n < 0 || n > 1 << 16 || (n > 0 && (!ranks || !a || !b || !scales)))
+    return fail(CREC_E_INVALID, "adapters_open: arguments");
+  try {
+    return open_adapters(device, model, model_bytes, n, ranks, static_cast<const uint16_t*>(a),
+                         static_cast<const uint16_t*>(b), scales, out, fail);
+  } catch (const std::bad_alloc&) {
+    return fail(CREC_E_NOMEM, "adapters_open: host memory");
+  } catch (const std::exception& e) {
+    return fail(CREC_E_INVALID, e.what());
+  }
+}
+
+int crec_adapters_close(crec_adapters* h) {
+  if (h) free_adapters(h);
+  return CREC_OK;
+}
+
+int crec_adapters_logits(crec_adapters* h, const void* x, int64_t x_pitch, int64_t rows, int lines,
+                         const int32_t* line_at, const int32_t* adapter, void* logits, int type, int64_t pitch,
+                         void* stream, char* error, size_t error_size) {
+  const Errors fail{error, error_size};
+  if (!h) return fail(CREC_E_INVALID, "adapters_logits: no handle");
+  if (!is_logits_type(type)) return fail(CREC_E_INVALID, "adapters_logits: the logits' type");
+  if (rows < 0 || rows > kMaxRows || lines < 0) return fail(CREC_E_INVALID, "adapters_logits: rows or lines");
+  if (x_pitch < h->k || x_pitch > kMaxPitch || x_pitch % 8 || reinterpret_cast<uintptr_t>(x) % 16)
+    return fail(CREC_E_INVALID, "adapters_logits: x 16-byte aligned, its pitch a multiple of 8 and at least K");
+  if (pitch < h->classes || pitch > kMaxPitch || reinterpret_cast<uintptr_t>(logits) % type_bytes(type))
+    return fail(CREC_E_INVALID, "adapters_logits: the logits' pitch or alignment");
+  if (lines == 0 || rows == 0) return CREC_OK;
+  if (!x || !line_at || !logits) return fail(CREC_E_INVALID, "adapters_logits: no x, line_at or logits");
+  OnDeviceOf on;
+  if (const cudaError_t e = on.to(h->device); e != cudaSuccess) return fail.cuda(e, "adapters_logits");
+  AdapterParams p{};
+  p.x = static_cast<const __half*>(x);
+  p.x_pitch = x_pitch;
+  p.rows = static_cast<int>(rows);
+  p.lines = lines;
+  p.k = h->k;
+  p.classes = h->classes;
+  p.line_at = line_at;
+  p.adapter = adapter;
+  p.w = h->w;
+  p.bias = h->bias;
+  p.adapters = h->adapters;
+  p.rank = h->rank;
+  p.a = h->a;
+  p.b = h->b;
+  p.scale = h->scale;
+  p.z = logits;
+  p.half = type == CREC_FP16;
+  p.pitch = pitch;
+  const dim3 grid(static_cast<unsigned>((rows + kHeadRows - 1) / kHeadRows), static_cast<unsigned>((h->classes + 255) / 256));
+  adapter_head_kernel<<<grid, 256, 0, static_cast<cudaStream_t>(stream)>>>(p);
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? CREC_OK : fail.cuda(e, "adapters_logits");
+}
+
+}  // extern "C"

@@ -53,6 +53,7 @@ extern "C" {
 
 #define CREC_INT8 0 /* the Q/DQ recognizer: int8 weights, uint8 activations, int32 sums */
 #define CREC_FP16 1 /* the float recognizer: float16 weights and activations, float32 sums */
+#define CREC_FP32 2 /* a type of logits (crec_line_logits, crec_adapters_logits) beside CREC_FP16; no recognizer's precision */
 
 typedef struct crec_handle crec_handle;
 
@@ -274,6 +275,115 @@ CREC_API int crec_ctc_head_blob(const void* file, size_t bytes, void* blob, size
                                 char* error, size_t error_size);
 CREC_API int crec_head_sweep(int device, int precision, const void* model, size_t model_bytes, int frames,
                              const void* x, int32_t* ids, float* probs, float* logits, int repeat, double* ms);
+
+/* ---------------------------------------------------------------- the logits of packed lines
+ *
+ * The calls below work on logits already in device memory, the frames of many lines end to end:
+ * frame f's classes at logits + f * pitch, line i's frames [line_at[i], line_at[i + 1]), class 0
+ * the CTC blank.  Every array is in device memory of one GPU, the one that holds the logits,
+ * whichever is current; the work is queued on `stream` (a cudaStream_t of that GPU; null its
+ * default stream) and not waited for; nothing is allocated and no scratch is shared, so calls may
+ * overlap on different streams, be captured into CUDA graphs and be replayed.  The small structs
+ * are read by the call itself.  No handle: a message for an error goes to error[0, error_size)
+ * (may be null).  line_at ascends from 0 or more to at most `rows`; rows outside
+ * [line_at[0], line_at[lines]) are neither read nor written.  What is only known on the GPU cannot
+ * be refused: a line_at that does not ascend gives unspecified results within the arrays.  No
+ * counterpart in the reference, whose decoders know no rules. */
+typedef struct crec_line_logits {
+  const void* logits; /* [rows][classes], rows `pitch` elements apart */
+  int type;           /* CREC_FP32 or CREC_FP16 */
+  int classes;        /* at least 1 */
+  int64_t pitch;      /* at least classes */
+  int64_t rows;       /* frames the array holds, at most 2^31 - 1 */
+  int lines;
+  const int32_t* line_at; /* [lines + 1] */
+} crec_line_logits;
+
+/* The lines' rules, each part left out where its pointer is null.  A frame's logit z of class c
+ * becomes, in this order, in float32 with every operation rounded on its own,
+ *   history: the line's ids history[history_at[i] .. history_at[i + 1]) (any order; those outside
+ *            [0, classes) count for nothing).  Where c is n > 0 times among them:
+ *            z = (z > 0 ? z / repeat[i] : z * repeat[i]) - (n * frequency[i] + presence[i])
+ *            (null: repeat 1, frequency 0, presence 0; repeat is positive)
+ *   bias:    z += bias[bias_of[i]][c] (bias_of null: table 0 for every line; an index outside
+ *            [0, biases): no bias).  A bias of -inf forbids its class.
+ *   allowed: -inf, whatever z was (NaN and infinities too), where bit c % 32 of word c / 32 of
+ *            set set_of[i] is 0 (set_of null: set 0 for every line; an index outside [0, sets):
+ *            every class allowed). */
+typedef struct crec_rules {
+  const int32_t* history;
+  const int32_t* history_at; /* [lines + 1], ascending from 0 or more */
+  const float* repeat;       /* [lines] */
+  const float* presence;     /* [lines] */
+  const float* frequency;    /* [lines] */
+  const float* bias;         /* [biases][classes] */
+  int biases;
+  const int32_t* bias_of;    /* [lines] */
+  const uint32_t* allowed;   /* [sets][(classes + 31) / 32] */
+  int sets;
+  const int32_t* set_of;     /* [lines] */
+} crec_rules;
+
+/* The logits under their lines' rules, written out for a decoder of the caller's own: out
+ * [rows][classes] of type out_type, rows out_pitch elements apart (CREC_FP16: rounded once, at
+ * the end).  out may be the logits themselves (same type and pitch) or lie beside them in rows of
+ * the same byte pitch; any other overlap is refused. */
+CREC_API int crec_logit_rules(const crec_line_logits* z, const crec_rules* rules, void* out, int out_type,
+                              int64_t out_pitch, void* stream, char* error, size_t error_size);
+
+/* crec_ctc_greedy of packed lines under their rules (null: none), the ruled logits never written.
+ * A frame's class is the lowest class of its highest ruled logit (the blank where the rules leave
+ * nothing), its probability 1 / sum_c exp(z_c - z_best); a character begins at a frame that is
+ * neither blank nor its line's previous frame's class, and its probability is the highest of its
+ * frames'.  Line i's counts[i] characters go to [line_at[i], line_at[i] + counts[i]) of ids, starts
+ * (its first frame, counted from the line's) and probs, the rest of the line's places get id -1,
+ * start -1, probability 0.  ids, starts and probs hold `rows` entries.  The ids, counts and
+ * starts are those of the definition exactly; the probabilities' sums are taken in float32 in
+ * another order than crec_ctc_greedy's.  A NaN that is allowed wins no frame and makes its
+ * frame's probability NaN, as does an allowed +inf. */
+CREC_API int crec_ctc_greedy_lines(const crec_line_logits* z, const crec_rules* rules, int32_t* counts, int32_t* ids,
+                                   int32_t* starts, float* probs, void* stream, char* error, size_t error_size);
+
+/* crec_candidates of packed lines under their rules (null: none): for each frame its topk likeliest
+ * classes but the blank, best first (ties to the lower class), ids [rows][topk], their
+ * log-probabilities logp [rows][topk] and the blank's, blank [rows], each (z - z_best) - ln sum_c
+ * exp(z_c - z_best).  Places beyond the classes that the rules leave: id -1, log-probability
+ * -inf.  0 <= topk <= min(16, classes - 1) (CREC_E_RANGE; crec_candidates clamps instead, but
+ * here the caller's arrays are laid out by topk). */
+CREC_API int crec_candidates_lines(const crec_line_logits* z, const crec_rules* rules, int topk, int32_t* ids,
+                                   float* logp, float* blank, void* stream, char* error, size_t error_size);
+
+/* ---------------------------------------------------------------- a head with adapters
+ *
+ * A recognizer's head (its last 1x1 convolution, K channels to `classes`) with low-rank adapters
+ * beside it, one a line: frame f of line i gets
+ *   z[f][c] = sum_k x[f][k] W[c][k] + b[c] + scale_a * sum_j (sum_k x[f][k] A_a[j][k]) B_a[c][j]
+ * with a = adapter[i] (outside [0, adapters): the head alone).  float16 features, weights and
+ * adapters, float32 sums (the adapters' inner sums too). */
+typedef struct crec_adapters crec_adapters;
+
+/* The channels and classes of the head of `model`: a float recognizer's blob, or
+ * crec_ctc_head_blob's.  CREC_E_MODEL where its last layer is no 1x1 convolution.  Needs no GPU. */
+CREC_API int crec_blob_head(const void* model, size_t model_bytes, int* k, int* classes, char* error, size_t error_size);
+
+/* The head of `model` (as crec_blob_head reads it, its weights rounded to float16) on GPU `device` with n adapters (0 or more): host arrays, ranks[i] the rank of adapter
+ * i (1..64), a its A matrices [ranks[i]][K] one after another, b its B matrices [classes][ranks[i]]
+ * one after another (float16 bits), scales [n].  K a multiple of 8, at most 512.  The arrays are
+ * copied.  Synchronous; the handle is not changed by the calls that use it. */
+CREC_API int crec_adapters_open(int device, const void* model, size_t model_bytes, int n, const int32_t* ranks,
+                                const void* a, const void* b, const float* scales, crec_adapters** out, char* error,
+                                size_t error_size);
+/* Waits for the GPU and frees the handle (null: nothing). CREC_E_TIMEOUT if a launch's bounded wait ran out. */
+CREC_API int crec_adapters_close(crec_adapters* h);
+/* The lines' logits.  Device arrays: x float16 [rows][K], rows x_pitch elements apart (x 16-byte
+ * aligned, x_pitch a multiple of 8), line_at [lines + 1] and adapter [lines] (null: the head
+ * alone), logits of type `type` (CREC_FP32 or CREC_FP16), rows `pitch` elements apart.  Queued on
+ * `stream`, nothing allocated, no scratch shared: calls may overlap, be captured and replayed.
+ * Rows outside [line_at[0], line_at[lines]) are not written.  Every wait inside is bounded: after
+ * one that ran out, the calls that follow (and crec_adapters_close) give CREC_E_TIMEOUT. */
+CREC_API int crec_adapters_logits(crec_adapters* h, const void* x, int64_t x_pitch, int64_t rows, int lines,
+                                  const int32_t* line_at, const int32_t* adapter, void* logits, int type,
+                                  int64_t pitch, void* stream, char* error, size_t error_size);
 
 /* The CUDA stream (a cudaStream_t) the handle's work runs on, for device-side timing. */
 CREC_API void* crec_stream(crec_handle* h);
