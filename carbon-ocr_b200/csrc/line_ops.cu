@@ -4,6 +4,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <cstdint>
 #include <cstdio>
@@ -72,7 +73,7 @@ constexpr int64_t kMaxPitch = int64_t{1} << 40;
 const char* lines_fault(const crec_line_logits* z) {
   if (!z) return "no logits";
   if (!is_logits_type(z->type)) return "the logits' type";
-  if (z->classes < 1) return "classes";
+  if (z->classes < 1 || z->classes > kMaxClasses) return "classes";
   if (z->rows < 0 || z->rows > kMaxRows || z->lines < 0) return "rows or lines";
   if (z->pitch < z->classes || z->pitch > kMaxPitch) return "pitch";
   if (z->lines > 0 && !z->line_at) return "no line_at";
@@ -115,16 +116,78 @@ LineParams line_params(const crec_line_logits* z, const crec_rules* r) {
   return p;
 }
 
-template <int kOp>
-cudaError_t launch_rows(const LineParams& p, int type, cudaStream_t s) {
-  const size_t smem = p.history ? static_cast<size_t>(p.classes) * 4 : 0;
-  auto* k = type == CREC_FP16 ? line_rows_kernel<kOp, __half> : line_rows_kernel<kOp, float>;
+// The number of SMs of the current device, asked once a device.
+cudaError_t sm_count(int* out) {
+  static std::atomic<int> known[64];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  int n = dev < 64 ? known[dev].load(std::memory_order_relaxed) : 0;
+  if (n == 0) {
+    e = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 64) known[dev].store(n, std::memory_order_relaxed);
+  }
+  *out = n;
+  return cudaSuccess;
+}
+
+template <int kOp, typename T, typename O, int V>
+cudaError_t launch_rows(LineParams& p, cudaStream_t s) {
+  int sms = 0;
+  cudaError_t e = sm_count(&sms);
+  if (e != cudaSuccess) return e;
+  // a team wide enough to hold a row; wider where the rows alone leave SMs without warps
+  int w = 1;
+  while (w < kMaxTeam && p.classes > w * kWarpClasses) w *= 2;
+  p.chunks = (p.classes + w * kWarpClasses - 1) / (w * kWarpClasses);
+  while (p.chunks == 1 && w < 8 && static_cast<long long>(p.rows) * w < 8ll * sms && p.classes > 64 * w) w *= 2;
+  p.warps = w;
+  p.slots = p.chunks * w;
+  p.span = ((p.classes + p.slots - 1) / p.slots + 32 * V - 1) / (32 * V) * (32 * V);
+  p.bias_wide = p.classes % 4 == 0 && reinterpret_cast<uintptr_t>(p.bias) % 16 == 0;
+  const int warps = w > 8 ? 16 : 8, teams = warps / w;
+  const long long resident = 16ll / w * sms;  // 16 warps an SM at 128 registers
+  p.team_rows = static_cast<int>(std::max(1ll, (p.rows + resident - 1) / resident));
+  size_t smem = teams * sizeof(RowSlots);
+  if (kOp == kOpCandidates) smem += (static_cast<size_t>(teams) * 2 * p.slots * kMaxTop + static_cast<size_t>(warps) * kShortList) * 8;
+  if (p.history) smem += static_cast<size_t>(warps) * p.span * 10;
+  auto* k = line_rows_kernel<kOp, T, O, V>;
   if (smem > 48 << 10) {
-    const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
     if (e != cudaSuccess) return e;
   }
-  k<<<static_cast<unsigned>(p.rows), kRowThreads, smem, s>>>(p);
+  const long long per_block = static_cast<long long>(p.team_rows) * teams;
+  k<<<static_cast<unsigned>((p.rows + per_block - 1) / per_block), warps * 32, smem, s>>>(p);
   return cudaGetLastError();
+}
+
+// Whether rows may be read or written `bytes` at a time.
+bool wide(const void* a, int64_t pitch, size_t element, size_t bytes) {
+  return reinterpret_cast<uintptr_t>(a) % bytes == 0 && pitch * element % bytes == 0;
+}
+
+template <int kOp>
+cudaError_t launch_decode(LineParams& p, int type, cudaStream_t s) {
+  if (type == CREC_FP16)
+    return wide(p.z, p.pitch, 2, 16) ? launch_rows<kOp, __half, float, 8>(p, s) : launch_rows<kOp, __half, float, 1>(p, s);
+  return wide(p.z, p.pitch, 4, 16) ? launch_rows<kOp, float, float, 4>(p, s) : launch_rows<kOp, float, float, 1>(p, s);
+}
+
+cudaError_t launch_rules(LineParams& p, int type, int out_type, cudaStream_t s) {
+  const bool w = wide(p.z, p.pitch, type_bytes(type), 16);
+  if (type == CREC_FP16) {
+    if (out_type == CREC_FP16)
+      return w && wide(p.out, p.out_pitch, 2, 16) ? launch_rows<kOpRules, __half, __half, 8>(p, s)
+                                                  : launch_rows<kOpRules, __half, __half, 1>(p, s);
+    return w && wide(p.out, p.out_pitch, 4, 16) ? launch_rows<kOpRules, __half, float, 8>(p, s)
+                                                : launch_rows<kOpRules, __half, float, 1>(p, s);
+  }
+  if (out_type == CREC_FP16)
+    return w && wide(p.out, p.out_pitch, 2, 8) ? launch_rows<kOpRules, float, __half, 4>(p, s)
+                                               : launch_rows<kOpRules, float, __half, 1>(p, s);
+  return w && wide(p.out, p.out_pitch, 4, 16) ? launch_rows<kOpRules, float, float, 4>(p, s)
+                                              : launch_rows<kOpRules, float, float, 1>(p, s);
 }
 
 // Whether the ruled logits may be written there: apart from the logits, exactly on them, or
@@ -286,9 +349,8 @@ int crec_logit_rules(const crec_line_logits* z, const crec_rules* rules, void* o
   if (const cudaError_t e = on.enter(z->logits); e != cudaSuccess) return fail.cuda(e, "logit_rules: the logits");
   LineParams p = line_params(z, rules);
   p.out = out;
-  p.out_half = out_type == CREC_FP16;
   p.out_pitch = out_pitch;
-  const cudaError_t e = launch_rows<kOpRules>(p, z->type, static_cast<cudaStream_t>(stream));
+  const cudaError_t e = launch_rules(p, z->type, out_type, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? CREC_OK : fail.cuda(e, "logit_rules");
 }
 
@@ -307,7 +369,7 @@ int crec_ctc_greedy_lines(const crec_line_logits* z, const crec_rules* rules, in
   p.starts = starts;
   p.probs = probs;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  cudaError_t e = p.rows > 0 ? launch_rows<kOpGreedy>(p, z->type, s) : cudaSuccess;
+  cudaError_t e = p.rows > 0 ? launch_decode<kOpGreedy>(p, z->type, s) : cudaSuccess;
   if (e == cudaSuccess) {
     collapse_lines_kernel<<<(p.lines + 3) / 4, 128, 0, s>>>(p);
     e = cudaGetLastError();
@@ -331,7 +393,7 @@ int crec_candidates_lines(const crec_line_logits* z, const crec_rules* rules, in
   p.probs = logp;
   p.blank = blank;
   p.topk = topk;
-  const cudaError_t e = launch_rows<kOpCandidates>(p, z->type, static_cast<cudaStream_t>(stream));
+  const cudaError_t e = launch_decode<kOpCandidates>(p, z->type, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? CREC_OK : fail.cuda(e, "candidates_lines");
 }
 

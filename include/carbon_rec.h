@@ -286,13 +286,13 @@ CREC_API int crec_head_sweep(int device, int precision, const void* model, size_
  * overlap on different streams, be captured into CUDA graphs and be replayed.  The small structs
  * are read by the call itself.  No handle: a message for an error goes to error[0, error_size)
  * (may be null).  line_at ascends from 0 or more to at most `rows`; rows outside
- * [line_at[0], line_at[lines]) are neither read nor written.  What is only known on the GPU cannot
+ * [line_at[0], line_at[lines]) are not written.  What is only known on the GPU cannot
  * be refused: a line_at that does not ascend gives unspecified results within the arrays.  No
  * counterpart in the reference, whose decoders know no rules. */
 typedef struct crec_line_logits {
   const void* logits; /* [rows][classes], rows `pitch` elements apart */
   int type;           /* CREC_FP32 or CREC_FP16 */
-  int classes;        /* at least 1 */
+  int classes;        /* 1 to 65536 */
   int64_t pitch;      /* at least classes */
   int64_t rows;       /* frames the array holds, at most 2^31 - 1 */
   int lines;
