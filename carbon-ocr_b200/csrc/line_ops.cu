@@ -12,6 +12,7 @@
 #include <memory>
 #include <new>
 #include <string>
+#include <utility>
 #include <vector>
 
 #include "../../include/carbon_rec.h"
@@ -132,34 +133,76 @@ cudaError_t sm_count(int* out) {
   return cudaSuccess;
 }
 
-template <int kOp, typename T, typename O, int V>
-cudaError_t launch_rows(LineParams& p, cudaStream_t s) {
+template <typename K>
+cudaError_t launch_on(K* k, const LineParams& p, long long blocks, int threads, size_t smem, cudaStream_t s) {
+  if (smem > 48 << 10) {
+    const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    if (e != cudaSuccess) return e;
+  }
+  k<<<static_cast<unsigned>(blocks), threads, smem, s>>>(p);
+  return cudaGetLastError();
+}
+
+// The launches with NV vectors of V classes a lane, NV the fewest in a list that hold `classes` in a
+// team's registers.
+template <int kOp, typename T, int V, int NV>
+cudaError_t decode_rows(LineParams& p, int sms, cudaStream_t s) {
+  using Row = WarpRow<T, V, NV>;
+  const int warps = p.warps > 8 ? 16 : 8, teams = warps / p.warps;
+  const long long resident = 16ll / p.warps * sms;  // 16 warps an SM at 128 registers
+  p.team_rows = static_cast<int>(std::max(1ll, (p.rows + resident - 1) / resident));
+  const long long per_block = static_cast<long long>(p.team_rows) * teams;
+  return launch_on(line_rows_kernel<kOp, T, V, NV>, p, (p.rows + per_block - 1) / per_block, warps * 32,
+                   teams * sizeof(TeamRow) + static_cast<size_t>(warps) * Row::kShared, s);
+}
+
+template <int kOp, typename T, int V, int... NV>
+cudaError_t decode_fit(LineParams& p, int need, int sms, cudaStream_t s, std::integer_sequence<int, NV...>) {
+  cudaError_t e = cudaErrorInvalidValue;
+  bool done = false;
+  ((!done && need <= NV ? (done = true, e = decode_rows<kOp, T, V, NV>(p, sms, s), 0) : 0), ...);
+  return e;
+}
+
+template <int kOp, typename T, int V>
+cudaError_t decode(LineParams& p, cudaStream_t s) {
   int sms = 0;
-  cudaError_t e = sm_count(&sms);
+  const cudaError_t e = sm_count(&sms);
   if (e != cudaSuccess) return e;
   // a team wide enough to hold a row; wider where the rows alone leave SMs without warps
   int w = 1;
-  while (w < kMaxTeam && p.classes > w * kWarpClasses) w *= 2;
-  p.chunks = (p.classes + w * kWarpClasses - 1) / (w * kWarpClasses);
-  while (p.chunks == 1 && w < 8 && static_cast<long long>(p.rows) * w < 8ll * sms && p.classes > 64 * w) w *= 2;
+  while (w < kMaxTeam && p.classes > w * 32 * kDecodeLane) w *= 2;
+  while (w < 8 && static_cast<long long>(p.rows) * w < 8ll * sms && p.classes > 64 * w) w *= 2;
   p.warps = w;
-  p.slots = p.chunks * w;
-  p.span = ((p.classes + p.slots - 1) / p.slots + 32 * V - 1) / (32 * V) * (32 * V);
-  p.bias_wide = p.classes % 4 == 0 && reinterpret_cast<uintptr_t>(p.bias) % 16 == 0;
-  const int warps = w > 8 ? 16 : 8, teams = warps / w;
-  const long long resident = 16ll / w * sms;  // 16 warps an SM at 128 registers
-  p.team_rows = static_cast<int>(std::max(1ll, (p.rows + resident - 1) / resident));
-  size_t smem = teams * sizeof(RowSlots);
-  if (kOp == kOpCandidates) smem += (static_cast<size_t>(teams) * 2 * p.slots * kMaxTop + static_cast<size_t>(warps) * kShortList) * 8;
-  if (p.history) smem += static_cast<size_t>(warps) * p.span * 10;
-  auto* k = line_rows_kernel<kOp, T, O, V>;
-  if (smem > 48 << 10) {
-    e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-    if (e != cudaSuccess) return e;
-  }
-  const long long per_block = static_cast<long long>(p.team_rows) * teams;
-  k<<<static_cast<unsigned>((p.rows + per_block - 1) / per_block), warps * 32, smem, s>>>(p);
-  return cudaGetLastError();
+  const int need = (p.classes + w * 32 * V - 1) / (w * 32 * V);
+  if constexpr (V == 4) return decode_fit<kOp, T, V>(p, need, sms, s, std::integer_sequence<int, 1, 2, 3, 4, 5, 6, 7, 8>{});
+  else if constexpr (V == 8) return decode_fit<kOp, T, V>(p, need, sms, s, std::integer_sequence<int, 1, 2, 3, 4>{});
+  else return decode_fit<kOp, T, V>(p, need, sms, s, std::integer_sequence<int, 4, 16, 32>{});
+}
+
+template <int kOp, typename T>
+cudaError_t decode_wide(LineParams& p, cudaStream_t s) {
+  return launch_on(wide_rows_kernel<kOp, T>, p, p.rows, 32 * kMaxTeam, sizeof(TeamRow) + static_cast<size_t>(kMaxTeam) * kWideSpan * 10, s);
+}
+
+template <typename T, typename O, int V, int NV>
+cudaError_t write_rows(LineParams& p, int sms, cudaStream_t s) {
+  using Row = WarpRow<T, V, NV>;
+  constexpr int kWarps = kRulesThreads / 32;
+  p.chunks = (p.classes + Row::kSpan - 1) / Row::kSpan;
+  const long long resident = 32ll * sms;  // 32 warps an SM at 64 registers
+  p.team_rows = static_cast<int>(std::max(1ll, (static_cast<long long>(p.rows) * p.chunks + resident - 1) / resident));
+  const long long units = (p.rows + p.team_rows - 1) / p.team_rows * static_cast<long long>(p.chunks);
+  return launch_on(logit_rules_kernel<T, O, V, NV>, p, (units + kWarps - 1) / kWarps, kRulesThreads,
+                   static_cast<size_t>(kWarps) * Row::kShared, s);
+}
+
+template <typename T, typename O, int V>
+cudaError_t write_rules(LineParams& p, cudaStream_t s) {
+  int sms = 0;
+  const cudaError_t e = sm_count(&sms);
+  if (e != cudaSuccess) return e;
+  return write_rows<T, O, V, kRulesLane / V>(p, sms, s);
 }
 
 // Whether rows may be read or written `bytes` at a time.
@@ -167,27 +210,29 @@ bool wide(const void* a, int64_t pitch, size_t element, size_t bytes) {
   return reinterpret_cast<uintptr_t>(a) % bytes == 0 && pitch * element % bytes == 0;
 }
 
+void bias_reads(LineParams& p) { p.bias_wide = p.classes % 4 == 0 && reinterpret_cast<uintptr_t>(p.bias) % 16 == 0; }
+
 template <int kOp>
 cudaError_t launch_decode(LineParams& p, int type, cudaStream_t s) {
+  bias_reads(p);
+  if (p.classes > kRegisterClasses) return type == CREC_FP16 ? decode_wide<kOp, __half>(p, s) : decode_wide<kOp, float>(p, s);
   if (type == CREC_FP16)
-    return wide(p.z, p.pitch, 2, 16) ? launch_rows<kOp, __half, float, 8>(p, s) : launch_rows<kOp, __half, float, 1>(p, s);
-  return wide(p.z, p.pitch, 4, 16) ? launch_rows<kOp, float, float, 4>(p, s) : launch_rows<kOp, float, float, 1>(p, s);
+    return wide(p.z, p.pitch, 2, 16) ? decode<kOp, __half, 8>(p, s) : decode<kOp, __half, 1>(p, s);
+  return wide(p.z, p.pitch, 4, 16) ? decode<kOp, float, 4>(p, s) : decode<kOp, float, 1>(p, s);
 }
 
 cudaError_t launch_rules(LineParams& p, int type, int out_type, cudaStream_t s) {
+  bias_reads(p);
+  p.in_place = p.z == p.out;
   const bool w = wide(p.z, p.pitch, type_bytes(type), 16);
   if (type == CREC_FP16) {
     if (out_type == CREC_FP16)
-      return w && wide(p.out, p.out_pitch, 2, 16) ? launch_rows<kOpRules, __half, __half, 8>(p, s)
-                                                  : launch_rows<kOpRules, __half, __half, 1>(p, s);
-    return w && wide(p.out, p.out_pitch, 4, 16) ? launch_rows<kOpRules, __half, float, 8>(p, s)
-                                                : launch_rows<kOpRules, __half, float, 1>(p, s);
+      return w && wide(p.out, p.out_pitch, 2, 16) ? write_rules<__half, __half, 8>(p, s) : write_rules<__half, __half, 1>(p, s);
+    return w && wide(p.out, p.out_pitch, 4, 16) ? write_rules<__half, float, 8>(p, s) : write_rules<__half, float, 1>(p, s);
   }
   if (out_type == CREC_FP16)
-    return w && wide(p.out, p.out_pitch, 2, 8) ? launch_rows<kOpRules, float, __half, 4>(p, s)
-                                               : launch_rows<kOpRules, float, __half, 1>(p, s);
-  return w && wide(p.out, p.out_pitch, 4, 16) ? launch_rows<kOpRules, float, float, 4>(p, s)
-                                              : launch_rows<kOpRules, float, float, 1>(p, s);
+    return w && wide(p.out, p.out_pitch, 2, 8) ? write_rules<float, __half, 4>(p, s) : write_rules<float, __half, 1>(p, s);
+  return w && wide(p.out, p.out_pitch, 4, 16) ? write_rules<float, float, 4>(p, s) : write_rules<float, float, 1>(p, s);
 }
 
 // Whether the ruled logits may be written there: apart from the logits, exactly on them, or

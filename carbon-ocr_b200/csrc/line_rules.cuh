@@ -41,11 +41,10 @@ struct LineParams {
   float* blank;
   int topk;
   // how the rows are shared out (line_ops.cu)
-  int warps;      // of a team
-  int span;       // classes a warp holds at once, a multiple of 32 * V
-  int chunks;     // passes over the classes a row takes
-  int slots;      // chunks * warps
+  int warps;      // of a team, a power of two
+  int chunks;     // rules: the spans that a row takes
   int team_rows;  // rows a team takes
+  int in_place;   // the ruled logits go where the logits are
   int bias_wide;  // the bias tables' rows may be read 16 bytes at a time
 };
 
@@ -115,32 +114,20 @@ __device__ __forceinline__ unsigned long long class_key(float v, int c) {
 
 // ---------------------------------------------------------------- the rows
 //
-// A team of `p.warps` warps takes rows one after another, each warp `p.span` (at most 1,024) of the
-// classes, a lane up to 32 of them in registers: V consecutive ones every 32 * V.  What a line's
-// rules add to those classes (its bias, -inf for what its set leaves out) stays in registers too, from
-// row to row until the line changes.  The classes of the line's history are taken out of that dense
-// pass (-inf, a bit in `gone`) and go through a list of their own, so that the division costs a few
-// lanes' work once a row and not every class a branch.
-//
-// A row is read once and held while its maximum is found and its sum of exp(z - best) taken; the
-// next row's loads are in flight meanwhile.
+// A warp holds a span of a row's classes in registers, a lane V consecutive ones every 32 * V.  What
+// the line's rules add to them (its bias, -inf for what its set leaves out) stays in registers too,
+// from row to row until the line changes.  The classes of the line's history are taken out of that
+// dense pass (-inf, a bit in `gone`) and go through a list of their own, so that the division costs a
+// few lanes' work once a row and not every class a branch.  The next row's loads are in flight while
+// a row is worked on.
 
-constexpr int kLaneClasses = 32;
-constexpr int kWarpClasses = 32 * kLaneClasses;
-constexpr int kMaxTeam = 16;                        // warps
-constexpr int kMaxClasses = 4 * kMaxTeam * kWarpClasses;
-constexpr int kMaxSlots = 4 * kMaxTeam;             // a row's partial results
+constexpr int kDecodeLane = 32;  // classes a lane holds in the decoders: 128 registers, 16 warps an SM
+constexpr int kRulesLane = 16;   // and where the ruled logits are written
+constexpr int kMaxTeam = 16;     // warps that share a row
+constexpr int kMaxClasses = 65536;
 constexpr int kMaxTop = 16;
-constexpr int kShortList = 64;  // candidates of a warp ranked at once
+constexpr int kShortList = 64;  // a row's candidates ranked at once
 constexpr float kLog2e = 1.44269504088896341f;
-
-// A warp's part of shared memory where there are histories: 10 bytes a class of its span.
-struct HadList {
-  uint32_t* count;  // [span] a class's count, then n * frequency + presence (its bits)
-  float* add;       // [span] an entry's bias, -inf where the set leaves it out
-  uint16_t* at;     // [span] the entries' classes within the span
-  int n;
-};
 
 template <typename T, int V>
 struct Raw;
@@ -223,6 +210,12 @@ __device__ __forceinline__ float warp_max(float v) {
   asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
   return m;
 }
+// The maximum, NaN where one of them is.
+__device__ __forceinline__ float warp_max_nan(float v) {
+  float m;
+  asm("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
+  return m;
+}
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
   for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -233,419 +226,637 @@ __device__ __forceinline__ unsigned long long warp_max_key(unsigned long long k)
   const uint32_t lo = __reduce_max_sync(0xffffffffu, static_cast<uint32_t>(k >> 32) == hi ? static_cast<uint32_t>(k) : 0u);
   return static_cast<unsigned long long>(hi) << 32 | lo;
 }
+// exp(v - best): the difference first, so that its rounding, not the logits' size, bounds the error.
 __device__ __forceinline__ float exp_less(float v, float best) { return ex2_approx(__fmul_rn(__fsub_rn(v, best), kLog2e)); }
 
-// A row's partial results, one a (chunk, warp) slot, two rows' worth (the next row's are written
-// while a warp joins this one's).
-struct RowSlots {
-  float best[2][kMaxSlots];
-  float sum[2][kMaxSlots];
-  int32_t arg[2][kMaxSlots];  // greedy: the lowest class of the slot's best
-  float blank[2];
+// A warp's part of shared memory: 10 bytes a class of its span.  add: what the rules add to each class
+// in the dense pass, -inf for what the set leaves out, for the history's classes and past the last
+// class; while a line's rules are set, the history's counts.  Then the entries: the history's classes
+// that are allowed, places within the span and n * frequency + presence.
+struct SpanRules {
+  float* add;
+  float* less;
+  uint16_t* at;
+  __device__ __forceinline__ SpanRules(uint8_t* shared, int span)
+      : add(reinterpret_cast<float*>(shared)), less(add + span), at(reinterpret_cast<uint16_t*>(less + span)) {}
 };
 
-// A warp's topk highest of its classes (v, the lanes' registers) and its n entries, as keys at
-// top[0, topk), highest first, 0 where nothing is left (-inf never is one).  The k-th highest of the
-// lanes' own maxima is at most the k-th highest of all, so only what reaches it is ranked: k keys
-// and a few more, unless many classes tie.
-template <int V, typename Entry>
-__device__ __forceinline__ void warp_top(int topk, int nv, const float (&v)[kLaneClasses], int n, Entry entry, int base,
-                                         int lane, unsigned long long* list, unsigned long long* top) {
-  constexpr int NV = kLaneClasses / V;
-  if (topk == 0) return;
-  float high = -INFINITY;
-#pragma unroll
+// A line's rules on the classes [base, base + 32 * V * NV) into a warp's SpanRules; the number of
+// entries.  *gone (rules written out only): bit j * V + i, this lane's class base + (j * 32 + lane) * V + i
+// is an entry.  Once a line: not inlined, its code out of the rows' way.
+template <int V, int NV>
+__device__ __noinline__ int set_rules(uint8_t* shared, int classes, int base, const int32_t* had, int n_had, float presence,
+                                      float frequency, const float* bias, bool bias_wide, const uint32_t* allowed, uint32_t* gone) {
+  constexpr int kSpan = 32 * V * NV;
+  const SpanRules s(shared, kSpan);
+  const int lane = threadIdx.x % 32;
+  uint32_t* count = reinterpret_cast<uint32_t*>(s.add);
+  int n = 0;
+  __syncwarp();
+  if (n_had > 0) {
+    for (int i = lane; i < kSpan; i += 32) count[i] = 0;
+    __syncwarp();
+    for (int k = lane; k < n_had; k += 32) {
+      const int c = had[k] - base;
+      if (c >= 0 && c < kSpan) atomicAdd(&count[c], 1u);
+    }
+    __syncwarp();
+  }
+  uint32_t mine = 0;
+#pragma unroll 1
   for (int j = 0; j < NV; ++j) {
-    if (j >= nv) break;
+    const int k = (j * 32 + lane) * V, c = base + k;
+    const uint32_t keep = allowed && c < classes ? allowed[c >> 5] >> (c & 31) : ~0u;
+    float b[V];
+    if (V > 1 && bias_wide && bias && c + V <= classes) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) high = fmaxf(high, v[j * V + i]);
-  }
-  for (int e = lane; e < n; e += 32) {
-    int c;
-    high = fmaxf(high, entry(e, c));
-  }
-  float s = high;  // sorted over the lanes, highest first
+      for (int i = 0; i < V / 4; ++i) {
+        const float4 f = *reinterpret_cast<const float4*>(bias + c + 4 * i);
+        b[4 * i] = f.x;
+        b[4 * i + 1] = f.y;
+        b[4 * i + 2] = f.z;
+        b[4 * i + 3] = f.w;
+      }
+    } else {
 #pragma unroll
-  for (int k = 2; k <= 32; k *= 2)
-#pragma unroll
-    for (int o = k / 2; o > 0; o /= 2) {
-      const float u = __shfl_xor_sync(0xffffffffu, s, o);
-      s = ((lane & o) == 0) == ((lane & k) == 0) ? fmaxf(s, u) : fminf(s, u);
+      for (int i = 0; i < V; ++i) b[i] = bias && c + i < classes ? bias[c + i] : 0.0f;
     }
-  const float reach = fmaxf(__shfl_sync(0xffffffffu, s, topk - 1), -3.402823466e38f);
-  int mine = 0;
-  if (high >= reach) {
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      if (j >= nv) break;
-#pragma unroll
-      for (int i = 0; i < V; ++i) mine += v[j * V + i] >= reach;
+    for (int i = 0; i < V; ++i) {
+      const uint32_t times = n_had > 0 ? count[k + i] : 0u;
+      const bool in = c + i < classes && (keep >> i & 1);
+      if (n_had > 0) {
+        const bool entry = times != 0 && in && b[i] != -INFINITY;
+        const unsigned m = __ballot_sync(0xffffffffu, entry);
+        if (entry) {
+          const int e = n + __popc(m & ((1u << lane) - 1));
+          s.at[e] = static_cast<uint16_t>(k + i);
+          s.less[e] = __fadd_rn(__fmul_rn(static_cast<float>(times), frequency), presence);
+          mine |= 1u << (j * V + i);
+        }
+        n += __popc(m);
+      }
+      b[i] = in && times == 0 ? b[i] : -INFINITY;
     }
-    for (int e = lane; e < n; e += 32) {
-      int c;
-      mine += entry(e, c) >= reach;
-    }
-  }
-  int upto = mine;
+    // a vector of the table is its lane's own: the counts that others have yet to read stay
 #pragma unroll
-  for (int o = 1; o < 32; o *= 2) {
-    const int u = __shfl_up_sync(0xffffffffu, upto, o);
-    if (lane >= o) upto += u;
+    for (int i = 0; i < V; ++i) s.add[k + i] = b[i];
   }
-  const int all = __shfl_sync(0xffffffffu, upto, 31);
-  if (all <= kShortList) {
-    if (mine) {
-      int at = upto - mine;
+  __syncwarp();
+  if (gone) *gone = mine;
+  return n;
+}
+
+// Entry e of the span's rules in the row at z (its classes from `base`).
+template <typename T>
+__device__ __noinline__ float far_entry(const T* z, const float* less, const uint16_t* at, int e, float repeat, const float* bias,
+                                        int base) {
+  const int k = at[e];
+  return __fadd_rn(penalised(load_logit(z + k), less[e], repeat), bias ? bias[base + k] : 0.0f);
+}
+
+// A warp's span of a row, and its line's rules on it.
+template <typename T, int V, int NV>
+struct WarpRow {
+  static constexpr int kLane = NV * V, kSpan = 32 * kLane;  // classes of a lane, of the warp
+  static constexpr int kShared = kSpan * 10;
+  int lane, base;  // the span's first class
+  int mine;        // whole vectors of this lane that hold classes
+  Raw<T, V> raw[NV];
+  LineRule l;
+  uint8_t* shared;
+  int n;  // entries
+  // The first 64 entries, two a lane, in registers: place, less, bias, the row's logit
+  int at[2];
+  float less[2], plus[2], z[2];
+
+  __device__ __forceinline__ void start(const LineParams& p, int base_, uint8_t* shared_) {
+    lane = threadIdx.x % 32;
+    base = base_;
+    shared = shared_;
+    l.first = l.end = 0;
+    n = 0;
+    at[0] = at[1] = 0;
+    const int left = p.classes - base - lane * V;
+    mine = left < V ? 0 : min(NV, (left - V) / (32 * V) + 1);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) raw[j].zero();
+  }
+  __device__ __forceinline__ const T* row(const LineParams& p, int r) const {
+    return static_cast<const T*>(p.z) + r * p.pitch + base;
+  }
+  __device__ __forceinline__ void load(const LineParams& p, int r) {
+    const T* q = row(p, r) + lane * V;
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+      if (j < mine) raw[j].load(q + j * 32 * V);
+    if (V > 1 && p.classes % V) {  // the vector that the last class lies in
+      const int left = p.classes - base - lane * V;
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
-        if (j >= nv) break;
-#pragma unroll
-        for (int i = 0; i < V; ++i)
-          if (v[j * V + i] >= reach) list[at++] = class_key(v[j * V + i], base + (j * 32 + lane) * V + i);
-      }
-      for (int e = lane; e < n; e += 32) {
-        int c;
-        const float x = entry(e, c);
-        if (x >= reach) list[at++] = class_key(x, c);
+        const int n_left = left - j * 32 * V;
+        if (n_left > 0 && n_left < V) raw[j].part(q + j * 32 * V, n_left);
       }
     }
-    __syncwarp();
-    const unsigned long long a = lane < all ? list[lane] : 0ull, b = lane + 32 < all ? list[lane + 32] : 0ull;
-    int ra = 0, rb = 0;
-    for (int i = 0; i < all; ++i) {
-      const unsigned long long k = list[i];
-      ra += k > a;
-      rb += k > b;
-    }
-    if (a && ra < topk) top[ra] = a;
-    if (b && rb < topk) top[rb] = b;
-    for (int q = all + lane; q < topk; q += 32) top[q] = 0ull;
-    __syncwarp();
-    return;
+    load_entries(p, r);
   }
-  // many alike: the highest key below the last one found, topk times
-  unsigned long long below = ~0ull;
-  for (int q = 0; q < topk; ++q) {
-    unsigned long long k = 0;
+  __device__ __forceinline__ void load_entries(const LineParams& p, int r) {
+    if (n == 0) return;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (lane + 32 * i < n) z[i] = load_logit(row(p, r) + at[i]);
+  }
+  // The rules of the line that row r (whose logits are loaded) lies in.
+  __device__ __forceinline__ void rules(const LineParams& p, int r, uint32_t* gone) {
+    n = set_rules<V, NV>(shared, p.classes, base, l.had, l.n_had, l.presence, l.frequency, l.bias, p.bias_wide, l.allowed, gone);
+    const SpanRules s(shared, kSpan);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if (lane + 32 * i >= n) continue;
+      at[i] = s.at[lane + 32 * i];
+      less[i] = s.less[lane + 32 * i];
+      plus[i] = l.bias ? l.bias[base + at[i]] : 0.0f;
+    }
+    load_entries(p, r);
+  }
+  // The dense pass.  Where a forbidden class holds NaN or +inf the sum with -inf is NaN; kCareful
+  // chooses instead of adding.
+  template <bool kCareful>
+  __device__ __forceinline__ void ruled(float (&v)[kLane]) const {
+    const float* t = reinterpret_cast<const float*>(shared) + lane * V;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      if (j >= nv) break;
+      float u[V], a[V];
+      raw[j].get(u);
+      if constexpr (V == 1) {
+        a[0] = t[j * 32];
+      } else {
+#pragma unroll
+        for (int i = 0; i < V / 4; ++i) {
+          const float4 f = *reinterpret_cast<const float4*>(t + j * 32 * V + 4 * i);
+          a[4 * i] = f.x;
+          a[4 * i + 1] = f.y;
+          a[4 * i + 2] = f.z;
+          a[4 * i + 3] = f.w;
+        }
+      }
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const unsigned long long u = v[j * V + i] >= reach ? class_key(v[j * V + i], base + (j * 32 + lane) * V + i) : 0ull;
-        if (u < below && u > k) k = u;
+        const float s = __fadd_rn(u[i], a[i]);
+        v[j * V + i] = kCareful && a[i] == -INFINITY ? a[i] : s;
       }
     }
-    for (int e = lane; e < n; e += 32) {
-      int c;
-      const float x = entry(e, c);
-      const unsigned long long u = x >= reach ? class_key(x, c) : 0ull;
-      if (u < below && u > k) k = u;
-    }
-    below = warp_max_key(k);
-    if (lane == 0) top[q] = below;
   }
+  // The ruled logits of this lane's first entries (-inf: none), taken before the next row's are loaded.
+  __device__ __forceinline__ void pair(float (&x)[2]) const {
+    x[0] = x[1] = -INFINITY;
+    if (n == 0) return;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (lane + 32 * i < n) x[i] = __fadd_rn(penalised(z[i], less[i], l.repeat), plus[i]);
+  }
+  // f(ruled logit, class) for each of this lane's entries in row r, x the first.
+  template <typename F>
+  __device__ __forceinline__ void entries(const LineParams& p, int r, const float (&x)[2], F f) const {
+    if (n == 0) return;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (lane + 32 * i < n) f(x[i], base + at[i]);
+    if (n <= 64) return;
+    const SpanRules s(shared, kSpan);
+#pragma unroll 1
+    for (int e = lane + 64; e < n; e += 32) f(far_entry(row(p, r), s.less, s.at, e, l.repeat, l.bias, base), base + s.at[e]);
+  }
+};
+
+// ---------------------------------------------------------------- the ruled logits
+
+constexpr int kRulesThreads = 128;
+
+// A warp takes `team_rows` rows of one span (of p.chunks); neighbouring warps the same rows' next span.
+template <typename T, typename O, int V, int NV>
+__global__ void __launch_bounds__(kRulesThreads, 8) logit_rules_kernel(const __grid_constant__ LineParams p) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  const int warp = threadIdx.x / 32;
+  const long long unit = static_cast<long long>(blockIdx.x) * (kRulesThreads / 32) + warp;
+  const long long r0 = unit / p.chunks * p.team_rows;
+  const int r1 = static_cast<int>(min(static_cast<long long>(p.rows), r0 + p.team_rows));
+  if (r0 >= r1) return;
+  using Row = WarpRow<T, V, NV>;
+  Row row;
+  row.start(p, static_cast<int>(unit % p.chunks) * Row::kSpan, smem + static_cast<size_t>(warp) * Row::kShared);
+  uint32_t gone = 0;
+  row.load(p, static_cast<int>(r0));
+  for (int r = static_cast<int>(r0); r < r1; ++r) {
+    bool some = true;
+    if (r < row.l.first || r >= row.l.end) {
+      some = find_line(p, r, row.lane, row.l);
+      if (some) row.rules(p, r, &gone);
+      else row.l.first = row.l.end = 0;
+    }
+    float v[Row::kLane], x[2];
+    row.template ruled<true>(v);
+    row.pair(x);
+    if (r + 1 < r1) row.load(p, r + 1);
+    if (!some) continue;
+    O* o = static_cast<O*>(p.out) + r * p.out_pitch;
+    // the dense stores cover the entries too (in place that would take the logits of those read only
+    // after them, past the 64 in registers: entries are then left out)
+    const bool spare = row.n > 64 && p.in_place;
+    const int c = row.base + row.lane * V;
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+      store_ruled<O, V>(o + c + j * 32 * V, v + j * V, spare ? gone >> (j * V) & ((1u << V) - 1) : 0u, p.classes - c - j * 32 * V);
+    if (row.n) {
+      __syncwarp();
+      row.entries(p, r, x, [&](float y, int k) {
+        if constexpr (sizeof(O) == 2) o[k] = __float2half_rn(y);
+        else o[k] = y;
+      });
+      __syncwarp();
+    }
+  }
+}
+
+// ---------------------------------------------------------------- the decoders
+//
+// A team of p.warps warps takes rows one after another, a warp a span of each.  First the maximum:
+// each lane's, then 32 groups' of lanes, then the team's best.  Then, against that best, the sums of
+// exp(z - best), joined in a fixed order.  Where the blank wins, the greedy decoder asks nothing more
+// of a row.
+
+// What a team's warps tell one another of a row, two rows' worth (a warp may be a row ahead).
+struct TeamRow {
+  float group[2][32];  // the highest of each group of lanes
+  float sum[2][kMaxTeam];
+  uint32_t arg[2][kMaxTeam];  // greedy: each warp's lowest class of the best
+  float blank[2];
+  int32_t listed[2];  // candidates: keys in the list
+  unsigned long long list[2][kShortList];
+  unsigned long long top[kMaxTeam];
+};
+
+// A span's classes but the blank in row z (its classes from `base`), from memory: what is seldom
+// needed, by whole warps.  f(ruled logit, class); a forbidden class is -inf whatever it holds.
+template <typename T, typename F>
+__device__ __forceinline__ void span_classes(const T* z, uint8_t* shared, int span, int base, int classes, int n, float repeat,
+                                             const float* bias, F f) {
+  const int lane = threadIdx.x % 32;
+  const SpanRules s(shared, span);
+#pragma unroll 1
+  for (int k = lane; k < span && base + k < classes; k += 32) {
+    const float a = s.add[k];
+    if (base + k != 0 && a != -INFINITY) f(__fadd_rn(load_logit(z + k), a), base + k);
+  }
+#pragma unroll 1
+  for (int e = lane; e < n; e += 32)
+    if (base + s.at[e] != 0) f(far_entry(z, s.less, s.at, e, repeat, bias, base), base + s.at[e]);
+}
+
+// The lane's sum of exp(z - best) where the dense pass met a NaN.
+template <typename T>
+__device__ __noinline__ float careful_sum(const T* z, uint8_t* shared, int span, int base, int classes, int n, float repeat,
+                                          const float* bias, float from) {
+  float sum = 0.0f;
+  span_classes(z, shared, span, base, classes, n, repeat, bias, [&](float y, int) { sum += exp_less(y, from); });
+  return sum;
+}
+
+// The warp's highest key below `below` (0: none).
+template <typename T>
+__device__ __noinline__ unsigned long long key_below(const T* z, uint8_t* shared, int span, int base, int classes, int n,
+                                                     float repeat, const float* bias, unsigned long long below) {
+  unsigned long long k = 0;
+  span_classes(z, shared, span, base, classes, n, repeat, bias, [&](float y, int c) {
+    const unsigned long long u = y > -INFINITY ? class_key(y, c) : 0ull;
+    if (u < below && u > k) k = u;
+  });
+  return warp_max_key(k);
+}
+
+// The k-th highest of 32 groups' maxima, one a lane: at most the k-th highest of all, so what reaches
+// it is k keys and a few more, unless many classes tie.  Never -inf.
+__device__ __forceinline__ float kth_group(float g, int k, int lane) {
+#pragma unroll
+  for (int m = 2; m <= 32; m *= 2)  // sorted over the lanes, highest first
+#pragma unroll
+    for (int o = m / 2; o > 0; o /= 2) {
+      const float u = __shfl_xor_sync(0xffffffffu, g, o);
+      g = ((lane & o) == 0) == ((lane & m) == 0) ? fmaxf(g, u) : fminf(g, u);
+    }
+  return fmaxf(__shfl_sync(0xffffffffu, g, k - 1), -3.402823466e38f);
+}
+
+__device__ __forceinline__ void list_key(TeamRow& t, int parity, float y, int c) {
+  const int at = atomicAdd(&t.listed[parity], 1);
+  if (at < kShortList) t.list[parity][at] = class_key(y, c);
+}
+
+// A row's candidates, by one warp: the listed keys ranked, the list emptied.  from: the row's best (0
+// where nothing is left), sum: of exp(z - from) over all classes.
+__device__ __forceinline__ void write_candidates(const LineParams& p, int r, int lane, TeamRow& t, int parity, float blank,
+                                                 float from, bool some, float sum) {
+  const float ln = some ? logf(sum) : sum;
+  const int all = t.listed[parity];
+  const unsigned long long a = lane < all ? t.list[parity][lane] : 0ull, b = lane + 32 < all ? t.list[parity][lane + 32] : 0ull;
+  int ra = 0, rb = 0;
+#pragma unroll 1
+  for (int i = 0; i < all; ++i) {
+    const unsigned long long k = t.list[parity][i];
+    ra += k > a;
+    rb += k > b;
+  }
+  const size_t o = static_cast<size_t>(r) * p.topk;
+  auto put = [&](unsigned long long k, int q) {
+    p.ids[o + q] = static_cast<int32_t>(0xffffffffu - static_cast<uint32_t>(k));
+    p.probs[o + q] = __fsub_rn(__fsub_rn(order_float(static_cast<uint32_t>(k >> 32)), from), ln);
+  };
+  if (a && ra < p.topk) put(a, ra);
+  if (b && rb < p.topk) put(b, rb);
+  if (lane >= all && lane < p.topk) {
+    p.ids[o + lane] = -1;
+    p.probs[o + lane] = -INFINITY;
+  }
+  if (lane == 0) p.blank[r] = __fsub_rn(__fsub_rn(blank, from), ln);
+  __syncwarp();
+  if (lane == 0) t.listed[parity] = 0;
   __syncwarp();
 }
 
-// A row's slots joined by one warp, and the row's results written.
-template <int kOp>
-__device__ __forceinline__ void join_slots(const LineParams& p, int r, int lane, const RowSlots& s, int parity,
-                                           const unsigned long long* tops) {
-  static_assert(kMaxSlots == 64, "two slots a lane");
-  const bool one = lane < p.slots, two = lane + 32 < p.slots;
-  const float b0 = one ? s.best[parity][lane] : -INFINITY, b1 = two ? s.best[parity][lane + 32] : -INFINITY;
-  const float best = warp_max(fmaxf(b0, b1));
-  const bool some = best > -INFINITY;
-  const float from = some ? best : 0.0f;
-  const float s0 = one ? s.sum[parity][lane] : 0.0f, s1 = two ? s.sum[parity][lane + 32] : 0.0f;
-  const float sum = warp_sum((b0 == -INFINITY ? s0 : s0 * exp_less(b0, from)) + (b1 == -INFINITY ? s1 : s1 * exp_less(b1, from)));
-  if constexpr (kOp == kOpGreedy) {
-    uint32_t c = one && b0 == best ? static_cast<uint32_t>(s.arg[parity][lane]) : 0x7fffffffu;
-    if (two && b1 == best) c = min(c, static_cast<uint32_t>(s.arg[parity][lane + 32]));
-    c = __reduce_min_sync(0xffffffffu, c);
-    if (lane == 0) {
-      p.ids[r] = some ? static_cast<int32_t>(c) : 0;
-      p.probs[r] = some ? __fdiv_rn(1.0f, sum) : sum;  // nothing left: 0 (NaN where one is allowed)
-    }
-  } else {
-    const float ln = some ? logf(sum) : sum;
-    unsigned long long mine = 0;
-    if (p.slots == 1) {
-      if (lane < p.topk) mine = tops[lane];
-    } else {
-      int at0 = 0, at1 = 0;
-      unsigned long long h0 = one && p.topk ? tops[lane * kMaxTop] : 0ull, h1 = two && p.topk ? tops[(lane + 32) * kMaxTop] : 0ull;
-      for (int q = 0; q < p.topk; ++q) {
-        const unsigned long long k = warp_max_key(h0 > h1 ? h0 : h1);
-        if (lane == q) mine = k;
-        if (k == 0) break;
-        if (h0 == k) h0 = ++at0 < p.topk ? tops[lane * kMaxTop + at0] : 0ull;
-        else if (h1 == k) h1 = ++at1 < p.topk ? tops[(lane + 32) * kMaxTop + at1] : 0ull;
-      }
-    }
-    if (lane < p.topk) {
-      const size_t o = static_cast<size_t>(r) * p.topk + lane;
-      p.ids[o] = mine ? static_cast<int32_t>(0xffffffffu - static_cast<uint32_t>(mine)) : -1;
-      p.probs[o] = mine ? __fsub_rn(__fsub_rn(order_float(static_cast<uint32_t>(mine >> 32)), from), ln) : -INFINITY;
-    }
-    if (lane == 0) p.blank[r] = __fsub_rn(__fsub_rn(s.blank[parity], from), ln);
-  }
-}
-
-template <int kOp, typename T, typename O, int V>
+template <int kOp, typename T, int V, int NV>
 __global__ void __launch_bounds__(512, 1) line_rows_kernel(const __grid_constant__ LineParams p) {
-  constexpr int NV = kLaneClasses / V;
+  using Row = WarpRow<T, V, NV>;
   extern __shared__ __align__(16) uint8_t smem[];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int team = warp / p.warps, w = warp % p.warps, teams = blockDim.x / 32 / p.warps;
-  const int nv = p.span / (32 * V);
-  // shared memory: the teams' slots, the warps' candidate lists, the warps' history lists
-  RowSlots* slots = reinterpret_cast<RowSlots*>(smem) + team;
-  unsigned long long* tops = reinterpret_cast<unsigned long long*>(smem + teams * sizeof(RowSlots)) +
-                             static_cast<size_t>(team) * 2 * p.slots * kMaxTop;  // [2][slots][kMaxTop]
-  uint8_t* after = smem + teams * sizeof(RowSlots) +
-                   (kOp == kOpCandidates ? static_cast<size_t>(teams) * 2 * p.slots * kMaxTop * 8 : 0);
-  unsigned long long* shortlist = reinterpret_cast<unsigned long long*>(after) + warp * kShortList;
-  if (kOp == kOpCandidates) after += static_cast<size_t>(blockDim.x / 32) * kShortList * 8;
-  HadList had;
-  had.n = 0;
-  had.count = reinterpret_cast<uint32_t*>(after + static_cast<size_t>(warp) * p.span * 10);
-  had.add = reinterpret_cast<float*>(had.count + p.span);
-  had.at = reinterpret_cast<uint16_t*>(had.add + p.span);
-  if (p.history) {
-    for (int i = lane; i < p.span; i += 32) had.count[i] = 0;
-    __syncwarp();
-  }
-
+  TeamRow& t = reinterpret_cast<TeamRow*>(smem)[team];
   const long long r0 = (static_cast<long long>(blockIdx.x) * teams + team) * p.team_rows;
   const int r1 = static_cast<int>(min(static_cast<long long>(p.rows), r0 + p.team_rows));
   if (r0 >= r1) return;
-
-  LineRule l;
-  l.first = l.end = 0;
-  float add[kLaneClasses];
-  uint32_t gone = 0;  // bit j * V + i: the class is in the line's history
-  Raw<T, V> raw[NV];
-  auto load = [&](int r, int base) {
-    const T* z = static_cast<const T*>(p.z) + r * p.pitch + base;
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      if (j >= nv) break;
-      const int c = (j * 32 + lane) * V, left = p.classes - base - c;
-      if (left >= V) raw[j].load(z + c);
-      else if (left > 0) raw[j].part(z + c, left);
-      else raw[j].zero();
-    }
+  auto team_sync = [&]() {
+    if (p.warps > 1) named_bar(1 + team, p.warps * 32);
+    else __syncwarp();
   };
-  // the line's rules on this warp's classes [base, base + span)
-  auto set_rules = [&](int base) {
-    for (int e = lane; e < had.n; e += 32) had.count[had.at[e]] = 0;
-    __syncwarp();
-    had.n = 0;
-    gone = 0;
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      if (j >= nv) break;
-      const int c = base + (j * 32 + lane) * V;
-      const uint32_t keep = l.allowed && c < p.classes ? l.allowed[c >> 5] >> (c & 31) : ~0u;
-      float b[V];
-      if (V > 1 && p.bias_wide && l.bias && c + V <= p.classes) {
-#pragma unroll
-        for (int i = 0; i < V / 4; ++i) {
-          const float4 f = *reinterpret_cast<const float4*>(l.bias + c + 4 * i);
-          b[4 * i] = f.x;
-          b[4 * i + 1] = f.y;
-          b[4 * i + 2] = f.z;
-          b[4 * i + 3] = f.w;
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i) b[i] = l.bias && c + i < p.classes ? l.bias[c + i] : 0.0f;
-      }
-#pragma unroll
-      for (int i = 0; i < V; ++i) add[j * V + i] = c + i < p.classes && (keep >> i & 1) ? b[i] : -INFINITY;
-    }
-    if (l.n_had <= 0) return;
-    for (int k0 = 0; k0 < l.n_had; k0 += 32) {
-      const int k = k0 + lane, c = k < l.n_had ? l.had[k] - base : -1;
-      const bool mine = c >= 0 && c < p.span && base + c < p.classes;
-      const bool first = mine && atomicAdd(&had.count[c], 1u) == 0;
-      const unsigned m = __ballot_sync(0xffffffffu, first);
-      if (first) had.at[had.n + __popc(m & ((1u << lane) - 1))] = static_cast<uint16_t>(c);
-      had.n += __popc(m);
-    }
-    if (had.n == 0) return;
-    __syncwarp();
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      if (j >= nv) break;
-#pragma unroll
-      for (int i = 0; i < V; ++i)
-        if (had.count[(j * 32 + lane) * V + i]) {
-          gone |= 1u << (j * V + i);
-          add[j * V + i] = -INFINITY;
-        }
-    }
-    __syncwarp();
-    for (int e = lane; e < had.n; e += 32) {
-      const int c = had.at[e];
-      const float n = static_cast<float>(had.count[c]);
-      had.count[c] = __float_as_uint(__fadd_rn(__fmul_rn(n, l.frequency), l.presence));
-      const bool keep = !l.allowed || (l.allowed[(base + c) >> 5] >> ((base + c) & 31) & 1);
-      had.add[e] = keep ? (l.bias ? l.bias[base + c] : 0.0f) : -INFINITY;
-    }
-    __syncwarp();
-  };
-  // entry e of the line's history in a row (z: its classes from `base`)
-  auto entry = [&](const T* z, int e) {
-    const int c = had.at[e];
-    const float a = had.add[e];
-    const float v = penalised(load_logit(z + c), __uint_as_float(had.count[c]), l.repeat);
-    return a == -INFINITY ? a : __fadd_rn(v, a);
-  };
-
+  if (kOp == kOpCandidates && w == 0 && lane < 2) t.listed[lane] = 0;  // seen by the other warps after a row's first barrier
+  Row row;
+  row.start(p, w * Row::kSpan, smem + teams * sizeof(TeamRow) + static_cast<size_t>(warp) * Row::kShared);
+  row.load(p, static_cast<int>(r0));
+  __syncwarp();
   int parity = 0;
-  const int base0 = w * p.span;
-  if (p.chunks == 1) load(static_cast<int>(r0), base0);
+#pragma unroll 1
   for (int r = static_cast<int>(r0); r < r1; ++r) {
-    bool fresh = false;
-    if (r < l.first || r >= l.end) {
-      fresh = true;
-      if (!find_line(p, r, lane, l)) {
-        l.first = l.end = 0;
-        if (p.chunks == 1 && r + 1 < r1) load(r + 1, base0);
-        continue;  // no line's row (every warp of the team finds the same)
-      }
+    bool found = true;
+    if (r < row.l.first || r >= row.l.end) {
+      found = find_line(p, r, lane, row.l);  // the same for every warp of the team
+      if (found) row.rules(p, r, nullptr);
+      else row.l.first = row.l.end = 0;
     }
-    for (int chunk = 0; chunk < p.chunks; ++chunk) {
-      const int base = (chunk * p.warps + w) * p.span;
-      const T* z = static_cast<const T*>(p.z) + r * p.pitch + base;
-      if (p.chunks > 1) load(r, base);
-      if (fresh || p.chunks > 1) set_rules(base);
-      float v[kLaneClasses];
-      auto ruled = [&](bool careful) {
+    float v[Row::kLane], x[2];
+    row.template ruled<false>(v);
+    row.pair(x);
+    if (r + 1 < r1) row.load(p, r + 1);
+    if (!found) continue;
+
+    // the maximum; the blank (class 0) is kept out of it and told apart
+    float blank = -INFINITY;
+    if (row.base == 0 && lane == 0) {
+      blank = reinterpret_cast<const float*>(row.shared)[0] == -INFINITY ? -INFINITY : v[0];
+      v[0] = -INFINITY;
+    }
+    float high;
+    {
+      float m[NV];
 #pragma unroll
-        for (int j = 0; j < NV; ++j) {
-          if (j >= nv) break;
-          float u[V];
-          raw[j].get(u);
+      for (int j = 0; j < NV; ++j) {
+        m[j] = v[j * V];
 #pragma unroll
-          for (int i = 0; i < V; ++i) {
-            const float a = add[j * V + i], s = __fadd_rn(u[i], a);
-            v[j * V + i] = careful && a == -INFINITY ? a : s;
-          }
+        for (int i = 1; i < V; ++i) m[j] = fmaxf(m[j], v[j * V + i]);
+      }
+#pragma unroll
+      for (int s = 1; s < NV; s *= 2)
+#pragma unroll
+        for (int j = 0; j + s < NV; j += 2 * s) m[j] = fmaxf(m[j], m[j + s]);
+      high = fmaxf(m[0], -INFINITY);
+    }
+    row.entries(p, r, x, [&](float y, int c) {
+      if (c == 0) blank = y;
+      else high = fmaxf(high, y);
+    });
+    float best;
+    if (p.warps == 1) {
+      best = warp_max(high);
+      blank = warp_max_nan(blank);
+    } else {
+      const int groups = 32 / p.warps;  // of each warp
+      float g = high;
+      for (int o = 16; o >= groups; o /= 2) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
+      if (lane < groups) t.group[parity][w * groups + lane] = g;
+      if (w == 0) {
+        blank = warp_max_nan(blank);
+        if (lane == 0) t.blank[parity] = blank;
+      }
+      team_sync();
+      best = warp_max(t.group[parity][lane]);
+      blank = t.blank[parity];
+    }
+    if (kOp == kOpGreedy && blank >= best) {  // a tie is the lower class's
+      if (w == 0 && lane == 0) {
+        p.ids[r] = 0;
+        p.probs[r] = 0.0f;
+      }
+      parity ^= 1;
+      continue;
+    }
+    best = fmaxf(best, blank);
+    const bool some = best > -INFINITY;
+    const float from = some ? best : 0.0f;
+
+    // the sum, and the lowest class of the best or what may be a candidate
+    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < Row::kLane; ++i) s[i % 4] += exp_less(v[i], from);
+    row.entries(p, r, x, [&](float y, int c) {
+      if (c != 0) s[0] += exp_less(y, from);
+    });
+    float sum = warp_sum((s[0] + s[1]) + (s[2] + s[3]));
+    if (sum != sum)  // a NaN or +inf met a -inf (or one is allowed)
+      sum = warp_sum(careful_sum(row.row(p, r), row.shared, Row::kSpan, row.base, p.classes, row.n, row.l.repeat, row.l.bias, from));
+    uint32_t arg = 0xffffffffu;
+    if constexpr (kOp == kOpGreedy) {
+      if (high == best) {
+        uint32_t c = 0xffffffffu;  // the place of the lane's lowest class of the best
+#pragma unroll
+        for (int j = NV - 1; j >= 0; --j)
+#pragma unroll
+          for (int i = V - 1; i >= 0; --i) c = v[j * V + i] == best ? j * 32 * V + i : c;
+        if (c != 0xffffffffu) arg = row.base + lane * V + c;
+        row.entries(p, r, x, [&](float y, int k) {
+          if (y == best && k != 0) arg = min(arg, static_cast<uint32_t>(k));
+        });
+      }
+      arg = __reduce_min_sync(0xffffffffu, arg);
+      if (p.warps > 1) {
+        if (lane == 0) {
+          t.sum[parity][w] = sum;
+          t.arg[parity][w] = arg;
         }
-      };
-      if constexpr (kOp == kOpRules) {
-        ruled(true);
-        if (p.chunks == 1 && r + 1 < r1) load(r + 1, base0);
-        O* o = static_cast<O*>(p.out) + r * p.out_pitch + base;
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-          if (j >= nv) break;
-          const int c = (j * 32 + lane) * V;
-          if (base + c < p.classes)
-            store_ruled<O, V>(o + c, v + j * V, gone >> (j * V) & ((1u << V) - 1), p.classes - base - c);
-        }
-        for (int e = lane; e < had.n; e += 32) {
-          const float x = entry(z, e);
-          if constexpr (sizeof(O) == 2) o[had.at[e]] = __float2half_rn(x);
-          else o[had.at[e]] = x;
-        }
-      } else {
-        // this warp's best, the sum of exp(z - best) and what else the row wants, into its slot
-        const int slot = chunk * p.warps + w;
-        float best, sum;
-        float m[NV];
-        float xm, xs;  // the entries': highest, and the sum of exp(x - xm)
-        int arg = 0;   // greedy: the lowest class of the best
-        for (bool careful = false;; careful = true) {
-          ruled(careful);
-          if (p.chunks == 1 && r + 1 < r1) load(r + 1, base0);
-#pragma unroll
-          for (int j = 0; j < NV; ++j) {
-            m[j] = -INFINITY;
-            if (j >= nv) continue;
-#pragma unroll
-            for (int i = 0; i < V; ++i) m[j] = fmaxf(m[j], v[j * V + i]);
-          }
-#pragma unroll
-          for (int s = NV / 2; s > 0; s /= 2)
-#pragma unroll
-            for (int j = 0; j < s; ++j) m[j] = fmaxf(m[j], m[j + s]);
-          xm = -INFINITY;
-          xs = 0.0f;
-          int xc = 0x7fffffff;
-          for (int e = lane; e < had.n; e += 32) {
-            const float x = entry(z, e);
-            if (x > xm) {
-              xs = __fadd_rn(xm == -INFINITY ? xs : __fmul_rn(xs, exp_less(xm, x)), 1.0f);
-              xm = x;
-              xc = base + had.at[e];
-            } else if (x != -INFINITY) {
-              if (x == xm) xc = min(xc, base + had.at[e]);
-              xs = __fadd_rn(xs, exp_less(x, xm));
-            }
-          }
-          best = warp_max(fmaxf(m[0], xm));
-          const float from = best == -INFINITY ? 0.0f : best;
-          float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-          for (int j = 0; j < NV; ++j) {
-            if (j >= nv) break;
-#pragma unroll
-            for (int i = 0; i < V; ++i) s[(j * V + i) % 4] += exp_less(v[j * V + i], from);
-          }
-          sum = (s[0] + s[1]) + (s[2] + s[3]);
-          if (had.n) sum += xm == -INFINITY ? xs : xs * exp_less(xm, from);
-          sum = warp_sum(sum);
-          if constexpr (kOp == kOpGreedy) {
-            int c = xm == best ? xc : 0x7fffffff;
-            if (m[0] == best) {
-#pragma unroll
-              for (int j = NV - 1; j >= 0; --j) {
-                if (j >= nv) continue;
-#pragma unroll
-                for (int i = V - 1; i >= 0; --i)
-                  if (v[j * V + i] == best) c = min(c, base + (j * 32 + lane) * V + i);
-              }
-            }
-            arg = static_cast<int>(__reduce_min_sync(0xffffffffu, static_cast<uint32_t>(c)));
-          }
-          // a NaN or +inf met a -inf (or is allowed): once more, choosing instead of adding
-          if (careful || sum == sum) break;
-          load(r, base);
+        team_sync();
+      }
+      if ((r & (p.warps - 1)) == w) {  // joined by one warp, another each row
+        if (p.warps > 1) {
+          sum = warp_sum(lane < p.warps ? t.sum[parity][lane] : 0.0f);
+          arg = __reduce_min_sync(0xffffffffu, lane < p.warps ? t.arg[parity][lane] : 0xffffffffu);
         }
         if (lane == 0) {
-          slots->best[parity][slot] = best;
-          slots->sum[parity][slot] = sum;
-          slots->arg[parity][slot] = arg;
-        }
-        if constexpr (kOp == kOpCandidates) {
-          if (base == 0) {  // the blank: noted, and out of the candidates
-            if (lane == 0) {
-              slots->blank[parity] = v[0];
-              v[0] = -INFINITY;
-            }
-            __syncwarp();
-            for (int e = lane; e < had.n; e += 32)
-              if (had.at[e] == 0) slots->blank[parity] = entry(z, e);
-            __syncwarp();
-          }
-          warp_top<V>(p.topk, nv, v, had.n, [&](int e, int& c) {
-            c = base + had.at[e];
-            return c == 0 ? -INFINITY : entry(z, e);
-          }, base, lane, shortlist, tops + (static_cast<size_t>(parity) * p.slots + slot) * kMaxTop);
+          p.ids[r] = static_cast<int32_t>(arg);
+          p.probs[r] = __fdiv_rn(1.0f, sum + exp_less(blank, from));
         }
       }
+    } else {
+      if (p.topk > 0) {
+        const float reach = kth_group(p.warps == 1 ? high : t.group[parity][lane], p.topk, lane);
+        if (high >= reach) {
+          uint32_t m = 0;
+#pragma unroll
+          for (int i = 0; i < Row::kLane; ++i) m |= static_cast<uint32_t>(v[i] >= reach) << i;
+          while (m) {  // few: the logit read again rather than kept where an index can reach it
+            const int i = __ffs(m) - 1, k = (i / V * 32 + lane) * V + i % V;
+            m &= m - 1;
+            list_key(t, parity, __fadd_rn(load_logit(row.row(p, r) + k), reinterpret_cast<const float*>(row.shared)[k]), row.base + k);
+          }
+          row.entries(p, r, x, [&](float y, int k) {
+            if (y >= reach && k != 0) list_key(t, parity, y, k);
+          });
+        }
+      }
+      if (lane == 0) t.sum[parity][w] = sum;
+      team_sync();
+      if (t.listed[parity] > kShortList) {  // many alike: the highest key below the last one found, topk times
+        unsigned long long below = ~0ull;
+#pragma unroll 1
+        for (int q = 0; q < p.topk; ++q) {
+          unsigned long long k =
+              key_below(row.row(p, r), row.shared, Row::kSpan, row.base, p.classes, row.n, row.l.repeat, row.l.bias, below);
+          if (p.warps > 1) {
+            if (lane == 0) t.top[w] = k;
+            team_sync();
+            k = warp_max_key(lane < p.warps ? t.top[lane] : 0ull);
+            team_sync();
+          }
+          below = k;
+          if (w == 0 && lane == 0) {
+            t.list[parity][q] = k;
+            t.listed[parity] = q + 1;
+          }
+        }
+        team_sync();
+      }
+      if ((r & (p.warps - 1)) == w) {
+        sum = warp_sum(lane < p.warps ? t.sum[parity][lane] : 0.0f) + exp_less(blank, from);
+        write_candidates(p, r, lane, t, parity, blank, from, some, sum);
+      }
     }
-    if constexpr (kOp != kOpRules) {
-      if (p.warps > 1) named_bar(1 + team, p.warps * 32);
-      else __syncwarp();
-      if (r % p.warps == w) join_slots<kOp>(p, r, lane, *slots, parity, tops + static_cast<size_t>(parity) * p.slots * kMaxTop);
-      parity ^= 1;
+    parity ^= 1;
+  }
+}
+
+// ---------------------------------------------------------------- rows that no team's registers hold
+//
+// More than kRegisterClasses classes: a block a row, its classes in passes of the same spans, each read
+// from memory as often as the row asks (and its rules set anew): right, not fast.
+
+constexpr int kRegisterClasses = kMaxTeam * 32 * kDecodeLane;
+constexpr int kWideSpan = 32 * kDecodeLane;
+
+template <int kOp, typename T>
+__global__ void __launch_bounds__(32 * kMaxTeam) wide_rows_kernel(const __grid_constant__ LineParams p) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  TeamRow& t = *reinterpret_cast<TeamRow*>(smem);
+  const int w = threadIdx.x / 32, lane = threadIdx.x % 32, r = blockIdx.x;
+  uint8_t* shared = smem + sizeof(TeamRow) + static_cast<size_t>(w) * kWideSpan * 10;
+  LineRule l;
+  if (!find_line(p, r, lane, l)) return;
+  if (threadIdx.x == 0) t.listed[0] = 0;
+  const T* z = static_cast<const T*>(p.z) + r * p.pitch;
+  // f(ruled logit, class) for this warp's classes but the blank
+  auto classes = [&](auto f) {
+#pragma unroll 1
+    for (int base = w * kWideSpan; base < p.classes; base += kMaxTeam * kWideSpan) {
+      const int n = set_rules<1, kDecodeLane>(shared, p.classes, base, l.had, l.n_had, l.presence, l.frequency, l.bias, false,
+                                              l.allowed, nullptr);
+      span_classes(z + base, shared, kWideSpan, base, p.classes, n, l.repeat, l.bias, f);
+      __syncwarp();
     }
+  };
+  float high = -INFINITY;
+  classes([&](float y, int) { high = fmaxf(high, y); });
+  for (int o = 16; o >= 2; o /= 2) high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, o));
+  if (lane < 2) t.group[0][w * 2 + lane] = high;
+  if (threadIdx.x == 0) {  // the blank
+    int times = 0;
+    for (int k = 0; k < l.n_had; ++k) times += l.had[k] == 0;
+    float y = load_logit(z);
+    if (times) y = penalised(y, __fadd_rn(__fmul_rn(static_cast<float>(times), l.frequency), l.presence), l.repeat);
+    if (l.bias) y = l.bias[0] == -INFINITY ? -INFINITY : __fadd_rn(y, l.bias[0]);
+    t.blank[0] = l.allowed && !(l.allowed[0] & 1u) ? -INFINITY : y;
+  }
+  __syncthreads();
+  const float blank = t.blank[0], others = warp_max(t.group[0][lane]), best = fmaxf(others, blank);
+  const bool some = best > -INFINITY;
+  const float from = some ? best : 0.0f;
+  if (kOp == kOpGreedy && blank >= others) {
+    if (threadIdx.x == 0) {
+      p.ids[r] = 0;
+      p.probs[r] = 0.0f;
+    }
+    return;
+  }
+  float sum = 0.0f;
+  uint32_t arg = 0xffffffffu;
+  const float reach = kOp == kOpCandidates && p.topk > 0 ? kth_group(t.group[0][lane], p.topk, lane) : INFINITY;
+  classes([&](float y, int c) {
+    sum += exp_less(y, from);
+    if constexpr (kOp == kOpGreedy) arg = y == best ? min(arg, static_cast<uint32_t>(c)) : arg;
+    else if (y >= reach && p.topk > 0) list_key(t, 0, y, c);
+  });
+  sum = warp_sum(sum);
+  arg = __reduce_min_sync(0xffffffffu, arg);
+  if (lane == 0) {
+    t.sum[0][w] = sum;
+    t.arg[0][w] = arg;
+  }
+  __syncthreads();
+  if (kOp == kOpCandidates && t.listed[0] > kShortList) {
+    unsigned long long below = ~0ull;
+#pragma unroll 1
+    for (int q = 0; q < p.topk; ++q) {
+      unsigned long long k = 0;
+      classes([&](float y, int c) {
+        const unsigned long long u = y > -INFINITY ? class_key(y, c) : 0ull;
+        if (u < below && u > k) k = u;
+      });
+      k = warp_max_key(k);
+      if (lane == 0) t.top[w] = k;
+      __syncthreads();
+      below = warp_max_key(lane < kMaxTeam ? t.top[lane] : 0ull);
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        t.list[0][q] = below;
+        t.listed[0] = q + 1;
+      }
+    }
+    __syncthreads();
+  }
+  if (w != 0) return;
+  sum = warp_sum(lane < kMaxTeam ? t.sum[0][lane] : 0.0f) + exp_less(blank, from);
+  if constexpr (kOp == kOpGreedy) {
+    arg = __reduce_min_sync(0xffffffffu, lane < kMaxTeam ? t.arg[0][lane] : 0xffffffffu);
+    if (lane == 0) {
+      p.ids[r] = static_cast<int32_t>(arg);
+      p.probs[r] = __fdiv_rn(1.0f, sum);
+    }
+  } else {
+    write_candidates(p, r, lane, t, 0, blank, from, some, sum);
   }
 }
 
