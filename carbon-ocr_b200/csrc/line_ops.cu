@@ -143,24 +143,32 @@ cudaError_t launch_on(K* k, const LineParams& p, long long blocks, int threads, 
   return cudaGetLastError();
 }
 
+// Blocks that an SM holds at once (227 KB of shared memory, 1 KB of it each block's own; 64 K registers).
+int blocks_an_sm(size_t smem, int warps, int registers) {
+  return std::max(1, std::min(static_cast<int>((228 << 10) / (smem + 1024)), 65536 / (registers * 32 * warps)));
+}
+
 // The launches with NV vectors of V classes a lane, NV the fewest in a list that hold `classes` in a
 // team's registers.
-template <int kOp, typename T, int V, int NV>
+constexpr int kAloneWarps = 2;  // of a block whose warps take rows alone
+
+template <int kOp, typename T, int V, int NV, bool kTeam>
 cudaError_t decode_rows(LineParams& p, int sms, cudaStream_t s) {
   using Row = WarpRow<T, V, NV>;
-  const int warps = p.warps > 8 ? 16 : 8, teams = warps / p.warps;
-  const long long resident = 16ll / p.warps * sms;  // 16 warps an SM at 128 registers
+  constexpr size_t kTeamRow = kTeam || kOp == kOpCandidates ? sizeof(TeamRow) : 0;
+  const int warps = kTeam ? p.warps : kAloneWarps, teams = kTeam ? 1 : warps;
+  const size_t smem = teams * kTeamRow + static_cast<size_t>(warps) * Row::kShared;
+  const long long resident = blocks_an_sm(smem, warps, 128) * static_cast<long long>(teams) * sms;
   p.team_rows = static_cast<int>(std::max(1ll, (p.rows + resident - 1) / resident));
   const long long per_block = static_cast<long long>(p.team_rows) * teams;
-  return launch_on(line_rows_kernel<kOp, T, V, NV>, p, (p.rows + per_block - 1) / per_block, warps * 32,
-                   teams * sizeof(TeamRow) + static_cast<size_t>(warps) * Row::kShared, s);
+  return launch_on(line_rows_kernel<kOp, T, V, NV, kTeam>, p, (p.rows + per_block - 1) / per_block, warps * 32, smem, s);
 }
 
 template <int kOp, typename T, int V, int... NV>
 cudaError_t decode_fit(LineParams& p, int need, int sms, cudaStream_t s, std::integer_sequence<int, NV...>) {
   cudaError_t e = cudaErrorInvalidValue;
   bool done = false;
-  ((!done && need <= NV ? (done = true, e = decode_rows<kOp, T, V, NV>(p, sms, s), 0) : 0), ...);
+  ((!done && need <= NV ? (done = true, e = p.warps > 1 ? decode_rows<kOp, T, V, NV, true>(p, sms, s) : decode_rows<kOp, T, V, NV, false>(p, sms, s), 0) : 0), ...);
   return e;
 }
 
@@ -190,11 +198,11 @@ cudaError_t write_rows(LineParams& p, int sms, cudaStream_t s) {
   using Row = WarpRow<T, V, NV>;
   constexpr int kWarps = kRulesThreads / 32;
   p.chunks = (p.classes + Row::kSpan - 1) / Row::kSpan;
-  const long long resident = 32ll * sms;  // 32 warps an SM at 64 registers
+  const size_t smem = static_cast<size_t>(kWarps) * Row::kShared;
+  const long long resident = blocks_an_sm(smem, kWarps, 64) * static_cast<long long>(kWarps) * sms;
   p.team_rows = static_cast<int>(std::max(1ll, (static_cast<long long>(p.rows) * p.chunks + resident - 1) / resident));
   const long long units = (p.rows + p.team_rows - 1) / p.team_rows * static_cast<long long>(p.chunks);
-  return launch_on(logit_rules_kernel<T, O, V, NV>, p, (units + kWarps - 1) / kWarps, kRulesThreads,
-                   static_cast<size_t>(kWarps) * Row::kShared, s);
+  return launch_on(logit_rules_kernel<T, O, V, NV>, p, (units + kWarps - 1) / kWarps, kRulesThreads, smem, s);
 }
 
 template <typename T, typename O, int V>

@@ -129,34 +129,34 @@ constexpr int kMaxTop = 16;
 constexpr int kShortList = 64;  // a row's candidates ranked at once
 constexpr float kLog2e = 1.44269504088896341f;
 
-template <typename T, int V>
-struct Raw;
-template <>
-struct Raw<float, 4> {
-  float4 r;
-  __device__ __forceinline__ void zero() { r = make_float4(0.0f, 0.0f, 0.0f, 0.0f); }
-  __device__ __forceinline__ void load(const float* z) { r = *reinterpret_cast<const float4*>(z); }
-  __device__ __forceinline__ void part(const float* z, int n) {
-    r = make_float4(z[0], n > 1 ? z[1] : 0.0f, n > 2 ? z[2] : 0.0f, 0.0f);
+// `bytes` (4, 8 or 16, both ends aligned to them) to shared memory without waiting; past `valid` zeros.
+template <int kBytes>
+__device__ __forceinline__ void copy_async(void* shared, const void* global, int valid) {
+  if constexpr (kBytes == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(shared)), "l"(global), "r"(valid) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(smem_u32(shared)), "l"(global), "n"(kBytes), "r"(valid)
+                 : "memory");
+}
+__device__ __forceinline__ void copy_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+// V logits from shared memory as float32.
+template <int V>
+__device__ __forceinline__ void get_logits(const float* z, float* v) {
+  if constexpr (V == 4) {
+    const float4 f = *reinterpret_cast<const float4*>(z);
+    v[0] = f.x;
+    v[1] = f.y;
+    v[2] = f.z;
+    v[3] = f.w;
+  } else {
+    v[0] = z[0];
   }
-  __device__ __forceinline__ void get(float* v) const {
-    v[0] = r.x;
-    v[1] = r.y;
-    v[2] = r.z;
-    v[3] = r.w;
-  }
-};
-template <>
-struct Raw<__half, 8> {
-  uint4 r;
-  __device__ __forceinline__ void zero() { r = make_uint4(0, 0, 0, 0); }
-  __device__ __forceinline__ void load(const __half* z) { r = *reinterpret_cast<const uint4*>(z); }
-  __device__ __forceinline__ void part(const __half* z, int n) {
-    const unsigned short* u = reinterpret_cast<const unsigned short*>(z);
-    auto two = [&](int i) { return (i < n ? static_cast<uint32_t>(u[i]) : 0u) | (i + 1 < n ? static_cast<uint32_t>(u[i + 1]) << 16 : 0u); };
-    r = make_uint4(two(0), two(2), two(4), two(6));
-  }
-  __device__ __forceinline__ void get(float* v) const {
+}
+template <int V>
+__device__ __forceinline__ void get_logits(const __half* z, float* v) {
+  if constexpr (V == 8) {
+    const uint4 r = *reinterpret_cast<const uint4*>(z);
     const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -166,16 +166,10 @@ struct Raw<__half, 8> {
       v[2 * i] = f.x;
       v[2 * i + 1] = f.y;
     }
+  } else {
+    v[0] = __half2float(z[0]);
   }
-};
-template <typename T>
-struct Raw<T, 1> {
-  T r;
-  __device__ __forceinline__ void zero() { memset(&r, 0, sizeof r); }
-  __device__ __forceinline__ void load(const T* z) { r = *z; }
-  __device__ __forceinline__ void part(const T* z, int) { r = *z; }
-  __device__ __forceinline__ void get(float* v) const { v[0] = load_logit(&r); }
-};
+}
 
 // V ruled logits written at o, those in `gone` (a bit each) left to the list.
 template <typename O, int V>
@@ -226,8 +220,32 @@ __device__ __forceinline__ unsigned long long warp_max_key(unsigned long long k)
   const uint32_t lo = __reduce_max_sync(0xffffffffu, static_cast<uint32_t>(k >> 32) == hi ? static_cast<uint32_t>(k) : 0u);
   return static_cast<unsigned long long>(hi) << 32 | lo;
 }
-// exp(v - best): the difference first, so that its rounding, not the logits' size, bounds the error.
-__device__ __forceinline__ float exp_less(float v, float best) { return ex2_approx(__fmul_rn(__fsub_rn(v, best), kLog2e)); }
+// exp(v - best) times a factor near 1 that is the same for all of a row's classes: 2^(v log2 e - c), c
+// the rounded best * log2 e, in one fused step.  What is made of a row's sums is divided by best's own
+// exp_less, which takes the factor out again, and with it the rounding of c.
+__device__ __forceinline__ float exp_less(float v, float c) { return ex2_approx(__fmaf_rn(v, kLog2e, -c)); }
+
+// A row's best (0 where nothing is left) and what its sums are taken against.
+struct RowBase {
+  float best, c;
+  bool fits;  // c is finite; else (|best| past 2.3e38) the difference is taken first
+  __device__ __forceinline__ explicit RowBase(float b) {
+    best = b == -INFINITY ? 0.0f : b;
+    c = __fmul_rn(best, kLog2e);
+    fits = fabsf(c) < INFINITY;
+  }
+  __device__ __forceinline__ float term(float v) const { return fits ? exp_less(v, c) : ex2_approx(__fmul_rn(__fsub_rn(v, best), kLog2e)); }
+};
+
+// Two at a time on the packed FP32 pipe, each half rounded on its own.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n .reg .b64 a, b, c, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n mov.b64 c, {%6, %7};\n"
+      " fma.rn.f32x2 d, a, b, c;\n mov.b64 {%0, %1}, d;\n}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
 
 // A warp's part of shared memory: 10 bytes a class of its span.  add: what the rules add to each class
 // in the dense pass, -inf for what the set leaves out, for the history's classes and past the last
@@ -315,20 +333,19 @@ __device__ __noinline__ float far_entry(const T* z, const float* less, const uin
   return __fadd_rn(penalised(load_logit(z + k), less[e], repeat), bias ? bias[base + k] : 0.0f);
 }
 
-// A warp's span of a row, and its line's rules on it.
+// A warp's span of a row, and its line's rules on it.  Rows come through a place in shared memory:
+// while one is worked on, in registers, the next is on its way there.
 template <typename T, int V, int NV>
 struct WarpRow {
   static constexpr int kLane = NV * V, kSpan = 32 * kLane;  // classes of a lane, of the warp
-  static constexpr int kShared = kSpan * 10;
+  static constexpr int kShared = kSpan * (10 + sizeof(T));
   int lane, base;  // the span's first class
-  int mine;        // whole vectors of this lane that hold classes
-  Raw<T, V> raw[NV];
   LineRule l;
-  uint8_t* shared;
+  uint8_t* shared;  // SpanRules, then the rows
   int n;  // entries
-  // The first 64 entries, two a lane, in registers: place, less, bias, the row's logit
+  // The first 64 entries, two a lane, in registers: place, less, bias
   int at[2];
-  float less[2], plus[2], z[2];
+  float less[2], plus[2];
 
   __device__ __forceinline__ void start(const LineParams& p, int base_, uint8_t* shared_) {
     lane = threadIdx.x % 32;
@@ -336,38 +353,38 @@ struct WarpRow {
     shared = shared_;
     l.first = l.end = 0;
     n = 0;
-    at[0] = at[1] = 0;
-    const int left = p.classes - base - lane * V;
-    mine = left < V ? 0 : min(NV, (left - V) / (32 * V) + 1);
-#pragma unroll
-    for (int j = 0; j < NV; ++j) raw[j].zero();
+    // places past the last class stay 0 (their add is -inf)
+    for (int k = max(0, p.classes - base) + lane; k < kSpan; k += 32) place()[k] = T(0.0f);
+    __syncwarp();
   }
   __device__ __forceinline__ const T* row(const LineParams& p, int r) const {
     return static_cast<const T*>(p.z) + r * p.pitch + base;
   }
-  __device__ __forceinline__ void load(const LineParams& p, int r) {
-    const T* q = row(p, r) + lane * V;
-#pragma unroll
-    for (int j = 0; j < NV; ++j)
-      if (j < mine) raw[j].load(q + j * 32 * V);
-    if (V > 1 && p.classes % V) {  // the vector that the last class lies in
+  __device__ __forceinline__ T* place() const { return reinterpret_cast<T*>(shared + kSpan * 10); }
+  // Row r (where r < r1) on its way.
+  __device__ __forceinline__ void fetch(const LineParams& p, int r, int r1) {
+    if (r < r1) {
+      const T* z = row(p, r) + lane * V;
+      T* s = place() + lane * V;
       const int left = p.classes - base - lane * V;
+      if constexpr (V * sizeof(T) >= 4) {
 #pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        const int n_left = left - j * 32 * V;
-        if (n_left > 0 && n_left < V) raw[j].part(q + j * 32 * V, n_left);
+        for (int j = 0; j < NV; ++j)
+          if (j * 32 * V < left)
+            copy_async<V * sizeof(T)>(s + j * 32 * V, z + j * 32 * V, min(V, left - j * 32 * V) * static_cast<int>(sizeof(T)));
+      } else {
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+          if (j * 32 * V < left) s[j * 32 * V] = z[j * 32 * V];
       }
     }
-    load_entries(p, r);
   }
-  __device__ __forceinline__ void load_entries(const LineParams& p, int r) {
-    if (n == 0) return;
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-      if (lane + 32 * i < n) z[i] = load_logit(row(p, r) + at[i]);
+  __device__ __forceinline__ void arrived() const {
+    copy_wait_all();
+    __syncwarp();
   }
-  // The rules of the line that row r (whose logits are loaded) lies in.
-  __device__ __forceinline__ void rules(const LineParams& p, int r, uint32_t* gone) {
+  // The rules of the line that the row lies in.
+  __device__ __forceinline__ void rules(const LineParams& p, uint32_t* gone) {
     n = set_rules<V, NV>(shared, p.classes, base, l.had, l.n_had, l.presence, l.frequency, l.bias, p.bias_wide, l.allowed, gone);
     const SpanRules s(shared, kSpan);
 #pragma unroll
@@ -377,17 +394,17 @@ struct WarpRow {
       less[i] = s.less[lane + 32 * i];
       plus[i] = l.bias ? l.bias[base + at[i]] : 0.0f;
     }
-    load_entries(p, r);
   }
   // The dense pass.  Where a forbidden class holds NaN or +inf the sum with -inf is NaN; kCareful
   // chooses instead of adding.
   template <bool kCareful>
   __device__ __forceinline__ void ruled(float (&v)[kLane]) const {
     const float* t = reinterpret_cast<const float*>(shared) + lane * V;
+    const T* z = place() + lane * V;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       float u[V], a[V];
-      raw[j].get(u);
+      get_logits<V>(z + j * 32 * V, u);
       if constexpr (V == 1) {
         a[0] = t[j * 32];
       } else {
@@ -400,20 +417,29 @@ struct WarpRow {
           a[4 * i + 3] = f.w;
         }
       }
+      if constexpr (V == 1 || kCareful) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const float s = __fadd_rn(u[i], a[i]);
-        v[j * V + i] = kCareful && a[i] == -INFINITY ? a[i] : s;
+        for (int i = 0; i < V; ++i) {
+          const float s = __fadd_rn(u[i], a[i]);
+          v[j * V + i] = kCareful && a[i] == -INFINITY ? a[i] : s;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; i += 2) {
+          const float2 s = fadd2_rn(make_float2(u[i], u[i + 1]), make_float2(a[i], a[i + 1]));
+          v[j * V + i] = s.x;
+          v[j * V + i + 1] = s.y;
+        }
       }
     }
   }
-  // The ruled logits of this lane's first entries (-inf: none), taken before the next row's are loaded.
+  // The ruled logits of this lane's first entries (-inf: none).
   __device__ __forceinline__ void pair(float (&x)[2]) const {
     x[0] = x[1] = -INFINITY;
     if (n == 0) return;
 #pragma unroll
     for (int i = 0; i < 2; ++i)
-      if (lane + 32 * i < n) x[i] = __fadd_rn(penalised(z[i], less[i], l.repeat), plus[i]);
+      if (lane + 32 * i < n) x[i] = __fadd_rn(penalised(load_logit(place() + at[i]), less[i], l.repeat), plus[i]);
   }
   // f(ruled logit, class) for each of this lane's entries in row r, x the first.
   template <typename F>
@@ -446,18 +472,20 @@ __global__ void __launch_bounds__(kRulesThreads, 8) logit_rules_kernel(const __g
   Row row;
   row.start(p, static_cast<int>(unit % p.chunks) * Row::kSpan, smem + static_cast<size_t>(warp) * Row::kShared);
   uint32_t gone = 0;
-  row.load(p, static_cast<int>(r0));
+  row.fetch(p, static_cast<int>(r0), r1);
   for (int r = static_cast<int>(r0); r < r1; ++r) {
     bool some = true;
     if (r < row.l.first || r >= row.l.end) {
       some = find_line(p, r, row.lane, row.l);
-      if (some) row.rules(p, r, &gone);
+      if (some) row.rules(p, &gone);
       else row.l.first = row.l.end = 0;
     }
     float v[Row::kLane], x[2];
+    row.arrived();
     row.template ruled<true>(v);
     row.pair(x);
-    if (r + 1 < r1) row.load(p, r + 1);
+    __syncwarp();
+    row.fetch(p, r + 1, r1);
     if (!some) continue;
     O* o = static_cast<O*>(p.out) + r * p.out_pitch;
     // the dense stores cover the entries too (in place that would take the logits of those read only
@@ -480,8 +508,10 @@ __global__ void __launch_bounds__(kRulesThreads, 8) logit_rules_kernel(const __g
 
 // ---------------------------------------------------------------- the decoders
 //
-// A team of p.warps warps takes rows one after another, a warp a span of each.  First the maximum:
-// each lane's, then 32 groups' of lanes, then the team's best.  Then, against that best, the sums of
+// A team takes rows one after another, a warp a span of each: a warp alone (kTeam false), or a block of
+// p.warps of them (a named barrier for each of several teams a block would cost every block all 16 of
+// the hardware's, and with them occupancy).  First the maximum: each lane's, then 32 groups' of lanes,
+// then the team's best.  Then, against that best, the sums of
 // exp(z - best), joined in a fixed order.  Where the blank wins, the greedy decoder asks nothing more
 // of a row.
 
@@ -516,9 +546,10 @@ __device__ __forceinline__ void span_classes(const T* z, uint8_t* shared, int sp
 // The lane's sum of exp(z - best) where the dense pass met a NaN.
 template <typename T>
 __device__ __noinline__ float careful_sum(const T* z, uint8_t* shared, int span, int base, int classes, int n, float repeat,
-                                          const float* bias, float from) {
+                                          const float* bias, float best) {
+  const RowBase from(best);
   float sum = 0.0f;
-  span_classes(z, shared, span, base, classes, n, repeat, bias, [&](float y, int) { sum += exp_less(y, from); });
+  span_classes(z, shared, span, base, classes, n, repeat, bias, [&](float y, int) { sum += from.term(y); });
   return sum;
 }
 
@@ -552,11 +583,11 @@ __device__ __forceinline__ void list_key(TeamRow& t, int parity, float y, int c)
   if (at < kShortList) t.list[parity][at] = class_key(y, c);
 }
 
-// A row's candidates, by one warp: the listed keys ranked, the list emptied.  from: the row's best (0
-// where nothing is left), sum: of exp(z - from) over all classes.
+// A row's candidates, by one warp: the listed keys ranked, the list emptied.  sum: the terms of all
+// classes.
 __device__ __forceinline__ void write_candidates(const LineParams& p, int r, int lane, TeamRow& t, int parity, float blank,
-                                                 float from, bool some, float sum) {
-  const float ln = some ? logf(sum) : sum;
+                                                 const RowBase& from, bool some, float sum) {
+  const float ln = some ? logf(__fdiv_rn(sum, from.term(from.best))) : sum;
   const int all = t.listed[parity];
   const unsigned long long a = lane < all ? t.list[parity][lane] : 0ull, b = lane + 32 < all ? t.list[parity][lane + 32] : 0ull;
   int ra = 0, rb = 0;
@@ -569,7 +600,7 @@ __device__ __forceinline__ void write_candidates(const LineParams& p, int r, int
   const size_t o = static_cast<size_t>(r) * p.topk;
   auto put = [&](unsigned long long k, int q) {
     p.ids[o + q] = static_cast<int32_t>(0xffffffffu - static_cast<uint32_t>(k));
-    p.probs[o + q] = __fsub_rn(__fsub_rn(order_float(static_cast<uint32_t>(k >> 32)), from), ln);
+    p.probs[o + q] = __fsub_rn(__fsub_rn(order_float(static_cast<uint32_t>(k >> 32)), from.best), ln);
   };
   if (a && ra < p.topk) put(a, ra);
   if (b && rb < p.topk) put(b, rb);
@@ -577,44 +608,47 @@ __device__ __forceinline__ void write_candidates(const LineParams& p, int r, int
     p.ids[o + lane] = -1;
     p.probs[o + lane] = -INFINITY;
   }
-  if (lane == 0) p.blank[r] = __fsub_rn(__fsub_rn(blank, from), ln);
+  if (lane == 0) p.blank[r] = __fsub_rn(__fsub_rn(blank, from.best), ln);
   __syncwarp();
   if (lane == 0) t.listed[parity] = 0;
   __syncwarp();
 }
 
-template <int kOp, typename T, int V, int NV>
+template <int kOp, typename T, int V, int NV, bool kTeam>
 __global__ void __launch_bounds__(512, 1) line_rows_kernel(const __grid_constant__ LineParams p) {
   using Row = WarpRow<T, V, NV>;
   extern __shared__ __align__(16) uint8_t smem[];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int team = warp / p.warps, w = warp % p.warps, teams = blockDim.x / 32 / p.warps;
-  TeamRow& t = reinterpret_cast<TeamRow*>(smem)[team];
-  const long long r0 = (static_cast<long long>(blockIdx.x) * teams + team) * p.team_rows;
+  const int w = kTeam ? warp : 0, warps = kTeam ? p.warps : 1;
+  constexpr int kTeamRow = kTeam || kOp == kOpCandidates ? sizeof(TeamRow) : 0;  // (a warp alone and greedy: unused)
+  const long long team = kTeam ? blockIdx.x : static_cast<long long>(blockIdx.x) * (blockDim.x / 32) + warp;
+  TeamRow& t = *reinterpret_cast<TeamRow*>(smem + (kTeam ? 0 : warp * (kTeamRow + Row::kShared)));
+  const long long r0 = team * p.team_rows;
   const int r1 = static_cast<int>(min(static_cast<long long>(p.rows), r0 + p.team_rows));
   if (r0 >= r1) return;
   auto team_sync = [&]() {
-    if (p.warps > 1) named_bar(1 + team, p.warps * 32);
+    if constexpr (kTeam) __syncthreads();
     else __syncwarp();
   };
   if (kOp == kOpCandidates && w == 0 && lane < 2) t.listed[lane] = 0;  // seen by the other warps after a row's first barrier
   Row row;
-  row.start(p, w * Row::kSpan, smem + teams * sizeof(TeamRow) + static_cast<size_t>(warp) * Row::kShared);
-  row.load(p, static_cast<int>(r0));
-  __syncwarp();
+  row.start(p, w * Row::kSpan, reinterpret_cast<uint8_t*>(&t) + kTeamRow + w * Row::kShared);
+  row.fetch(p, static_cast<int>(r0), r1);
   int parity = 0;
 #pragma unroll 1
   for (int r = static_cast<int>(r0); r < r1; ++r) {
     bool found = true;
     if (r < row.l.first || r >= row.l.end) {
       found = find_line(p, r, lane, row.l);  // the same for every warp of the team
-      if (found) row.rules(p, r, nullptr);
+      if (found) row.rules(p, nullptr);
       else row.l.first = row.l.end = 0;
     }
     float v[Row::kLane], x[2];
+    row.arrived();
     row.template ruled<false>(v);
     row.pair(x);
-    if (r + 1 < r1) row.load(p, r + 1);
+    __syncwarp();
+    row.fetch(p, r + 1, r1);
     if (!found) continue;
 
     // the maximum; the blank (class 0) is kept out of it and told apart
@@ -643,11 +677,11 @@ __global__ void __launch_bounds__(512, 1) line_rows_kernel(const __grid_constant
       else high = fmaxf(high, y);
     });
     float best;
-    if (p.warps == 1) {
+    if constexpr (!kTeam) {
       best = warp_max(high);
       blank = warp_max_nan(blank);
     } else {
-      const int groups = 32 / p.warps;  // of each warp
+      const int groups = 32 / warps;  // of each warp
       float g = high;
       for (int o = 16; o >= groups; o /= 2) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
       if (lane < groups) t.group[parity][w * groups + lane] = g;
@@ -669,18 +703,21 @@ __global__ void __launch_bounds__(512, 1) line_rows_kernel(const __grid_constant
     }
     best = fmaxf(best, blank);
     const bool some = best > -INFINITY;
-    const float from = some ? best : 0.0f;
+    const RowBase from(best);
 
     // the sum, and the lowest class of the best or what may be a candidate
-    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    float2 s[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
-    for (int i = 0; i < Row::kLane; ++i) s[i % 4] += exp_less(v[i], from);
+    for (int i = 0; i < Row::kLane; i += 2) {
+      const float2 d = fma2(make_float2(v[i], v[i + 1]), make_float2(kLog2e, kLog2e), make_float2(-from.c, -from.c));
+      s[i / 2 % 2] = fadd2_rn(s[i / 2 % 2], make_float2(ex2_approx(d.x), ex2_approx(d.y)));
+    }
     row.entries(p, r, x, [&](float y, int c) {
-      if (c != 0) s[0] += exp_less(y, from);
+      if (c != 0) s[0].x += exp_less(y, from.c);
     });
-    float sum = warp_sum((s[0] + s[1]) + (s[2] + s[3]));
-    if (sum != sum)  // a NaN or +inf met a -inf (or one is allowed)
-      sum = warp_sum(careful_sum(row.row(p, r), row.shared, Row::kSpan, row.base, p.classes, row.n, row.l.repeat, row.l.bias, from));
+    float sum = warp_sum((s[0].x + s[0].y) + (s[1].x + s[1].y));
+    if (sum != sum || !from.fits)  // a NaN or +inf met a -inf (or one is allowed), or c overflowed
+      sum = warp_sum(careful_sum(row.row(p, r), row.shared, Row::kSpan, row.base, p.classes, row.n, row.l.repeat, row.l.bias, best));
     uint32_t arg = 0xffffffffu;
     if constexpr (kOp == kOpGreedy) {
       if (high == best) {
@@ -695,26 +732,26 @@ __global__ void __launch_bounds__(512, 1) line_rows_kernel(const __grid_constant
         });
       }
       arg = __reduce_min_sync(0xffffffffu, arg);
-      if (p.warps > 1) {
+      if constexpr (kTeam) {
         if (lane == 0) {
           t.sum[parity][w] = sum;
           t.arg[parity][w] = arg;
         }
         team_sync();
       }
-      if ((r & (p.warps - 1)) == w) {  // joined by one warp, another each row
-        if (p.warps > 1) {
-          sum = warp_sum(lane < p.warps ? t.sum[parity][lane] : 0.0f);
-          arg = __reduce_min_sync(0xffffffffu, lane < p.warps ? t.arg[parity][lane] : 0xffffffffu);
+      if (!kTeam || (r & (warps - 1)) == w) {  // joined by one warp, another each row
+        if constexpr (kTeam) {
+          sum = warp_sum(lane < warps ? t.sum[parity][lane] : 0.0f);
+          arg = __reduce_min_sync(0xffffffffu, lane < warps ? t.arg[parity][lane] : 0xffffffffu);
         }
         if (lane == 0) {
           p.ids[r] = static_cast<int32_t>(arg);
-          p.probs[r] = __fdiv_rn(1.0f, sum + exp_less(blank, from));
+          p.probs[r] = __fdiv_rn(from.term(best), sum + from.term(blank));
         }
       }
     } else {
       if (p.topk > 0) {
-        const float reach = kth_group(p.warps == 1 ? high : t.group[parity][lane], p.topk, lane);
+        const float reach = kth_group(!kTeam ? high : t.group[parity][lane], p.topk, lane);
         if (high >= reach) {
           uint32_t m = 0;
 #pragma unroll
@@ -737,10 +774,10 @@ __global__ void __launch_bounds__(512, 1) line_rows_kernel(const __grid_constant
         for (int q = 0; q < p.topk; ++q) {
           unsigned long long k =
               key_below(row.row(p, r), row.shared, Row::kSpan, row.base, p.classes, row.n, row.l.repeat, row.l.bias, below);
-          if (p.warps > 1) {
+          if constexpr (kTeam) {
             if (lane == 0) t.top[w] = k;
             team_sync();
-            k = warp_max_key(lane < p.warps ? t.top[lane] : 0ull);
+            k = warp_max_key(lane < warps ? t.top[lane] : 0ull);
             team_sync();
           }
           below = k;
@@ -751,8 +788,8 @@ __global__ void __launch_bounds__(512, 1) line_rows_kernel(const __grid_constant
         }
         team_sync();
       }
-      if ((r & (p.warps - 1)) == w) {
-        sum = warp_sum(lane < p.warps ? t.sum[parity][lane] : 0.0f) + exp_less(blank, from);
+      if (!kTeam || (r & (warps - 1)) == w) {
+        sum = warp_sum(lane < warps ? t.sum[parity][lane] : 0.0f) + from.term(blank);
         write_candidates(p, r, lane, t, parity, blank, from, some, sum);
       }
     }
@@ -803,7 +840,7 @@ __global__ void __launch_bounds__(32 * kMaxTeam) wide_rows_kernel(const __grid_c
   __syncthreads();
   const float blank = t.blank[0], others = warp_max(t.group[0][lane]), best = fmaxf(others, blank);
   const bool some = best > -INFINITY;
-  const float from = some ? best : 0.0f;
+  const RowBase from(best);
   if (kOp == kOpGreedy && blank >= others) {
     if (threadIdx.x == 0) {
       p.ids[r] = 0;
@@ -815,7 +852,7 @@ __global__ void __launch_bounds__(32 * kMaxTeam) wide_rows_kernel(const __grid_c
   uint32_t arg = 0xffffffffu;
   const float reach = kOp == kOpCandidates && p.topk > 0 ? kth_group(t.group[0][lane], p.topk, lane) : INFINITY;
   classes([&](float y, int c) {
-    sum += exp_less(y, from);
+    sum += from.term(y);
     if constexpr (kOp == kOpGreedy) arg = y == best ? min(arg, static_cast<uint32_t>(c)) : arg;
     else if (y >= reach && p.topk > 0) list_key(t, 0, y, c);
   });
@@ -848,12 +885,12 @@ __global__ void __launch_bounds__(32 * kMaxTeam) wide_rows_kernel(const __grid_c
     __syncthreads();
   }
   if (w != 0) return;
-  sum = warp_sum(lane < kMaxTeam ? t.sum[0][lane] : 0.0f) + exp_less(blank, from);
+  sum = warp_sum(lane < kMaxTeam ? t.sum[0][lane] : 0.0f) + from.term(blank);
   if constexpr (kOp == kOpGreedy) {
     arg = __reduce_min_sync(0xffffffffu, lane < kMaxTeam ? t.arg[0][lane] : 0xffffffffu);
     if (lane == 0) {
       p.ids[r] = static_cast<int32_t>(arg);
-      p.probs[r] = __fdiv_rn(1.0f, sum);
+      p.probs[r] = __fdiv_rn(from.term(best), sum);
     }
   } else {
     write_candidates(p, r, lane, t, 0, blank, from, some, sum);
