@@ -1,8 +1,19 @@
 // A head with low-rank adapters beside it (carbon_rec.h, crec_adapters_logits): frame f of line i,
-//   z[f][c] = sum_k x[f][k] W[c][k] + b[c] + scale_a * sum_j h[f][j] B_a[c][j]
-//   h[f][j] = sum_k x[f][k] A_a[j][k],  a = adapter[i]
+//   z[f][c] = sum_k x[f][k] W[c][k] + b[c] + sum_j h[f][j] B_a[c][j]
+//   h[f][j] = scale_a * sum_k x[f][k] A_a[j][k],  a = adapter[i]
+//
+// One tcgen05 kernel: a tile of 128 frames stays in shared memory while the weights stream past it,
+// N classes a chunk, into float32 accumulators in TMEM.  The adapters join in the same accumulators.
+// The frames of a tile may belong to many lines with many adapters; each distinct one (a slot) is a
+// few more MMAs whose output rows are masked to the slot's own (disable-output-lane), so no frame is
+// moved, and the cost goes with the distinct adapters of a tile, not its lines.  First h: every
+// slot's A rows as the B operand, all into the same columns of TMEM, a row keeping its own slot's.
+// Four warps scale it and put it back as an A operand, as two tf32 words whose sum holds 22 bits (h
+// rounded to float16 once would cost the logits 2^-11 of the adapter's part, and its range; B's
+// float16 values are tf32 values exactly).  Then each slot's B rows over each chunk's accumulators.
 #pragma once
 
+#include <cuda.h>
 #include <cuda_fp16.h>
 
 #include <cstdint>
@@ -13,22 +24,57 @@ namespace crec {
 
 constexpr int kMaxRank = 64;
 constexpr int kMaxHeadK = 512;
+constexpr int kAdapterChunk = 224;  // classes: two accumulators and 64 columns of h in 512 columns of TMEM
+constexpr int kAdapterStages = 8;   // at most
+constexpr int kAdapterThreads = 14 * 32;
 
 struct AdapterParams {
-  const __half* x;  // [rows][k], rows x_pitch apart
-  long long x_pitch;
-  int rows, lines, k, classes;
+  CUtensorMap x;  // [rows][k] float16, boxes of 64 x 128 rows
+  CUtensorMap w;  // [classes][k] float16, boxes of 64 x n
+  CUtensorMap a;  // [adapters][r16][k] float16, boxes of 64 x r16
+  CUtensorMap b;  // [adapters][classes][rank] float32, boxes of min(rank, 32) x n
+  int rows, lines, classes;
   const int32_t* line_at;
   const int32_t* adapter;  // null: the head alone
-  const __half* w;         // [classes][k]
-  const float* bias;       // [classes]
-  int adapters, rank;      // rank: the widest, what A and B are padded to
-  const __half* a;         // [adapters][rank][k]
-  const __half* b;         // [adapters][classes][rank]
-  const float* scale;      // [adapters]
+  int adapters;
+  const float* bias;   // [classes], zeros to a multiple of 256
+  const float* scale;  // [adapters]
   void* z;
-  int half;
   long long pitch;
+  int half;
+  int width;  // bytes that a row of z may be written at once: 32, 16, or an element's
+  // tiles
+  int n, chunks, splits, chunks_per;  // classes a chunk (a multiple of 16); a tile's chunks, in `splits` parts
+  int items;                          // tiles * splits
+  int nkb, last_steps;                // 64-channel blocks of x; MMA steps (16 channels) of the last
+  int rank, r16, rank_row;            // padded to 8, 16, 32 or 64; at least 16; bytes of a row of b's boxes
+  int a_stage_blocks;                 // blocks of an adapter's A rows that a stage takes
+  int stages;
+  uint32_t stage_bytes, h_bytes;  // h_bytes: of one of h's two words
+  int* err;
+  unsigned long long wait_ns;
+};
+
+// What the roles of a block know of a tile's frames.
+struct TileSlots {
+  int n;
+  int pad[3];
+  uint4 rows[128];  // each slot's frames, a bit each
+  int id[128];      // and its adapter
+  int slot[128];    // each frame's slot, -1 none, -2 not a line's frame
+  float scale[128];
+};
+
+struct AdapterShared {
+  uint64_t full[kAdapterStages], empty[kAdapterStages];
+  uint64_t a_full, a_empty, t_full[2], t_empty[2], h_full, h2_full, h2_empty, s_full[2], s_empty[2];
+  uint32_t tmem;
+  int failed;
+  TileSlots tile[2];
+  int which[128];
+  int first_slot[128];
+  int places[129];
+  int counts[4];
 };
 
 // The line of row r, or -1 outside [line_at[0], line_at[lines]).
@@ -43,56 +89,443 @@ __device__ __forceinline__ int line_of_row(const int32_t* line_at, int lines, in
   return lo;
 }
 
-constexpr int kHeadRows = 16;
+// The tile's slots, by the 128 threads of the h warps (thread t frame r0 + t), barrier 1 theirs.
+__device__ __forceinline__ void find_slots(const AdapterParams& p, AdapterShared& s, TileSlots& tile, int r0, int t) {
+  const int lane = t % 32, q = t / 32, r = r0 + t;
+  int id = -2;
+  if (p.lines > 0) {
+    const int first = p.line_at[0], end = p.line_at[p.lines];
+    // the last line that begins at or before the tile, by warps of 32 probes
+    int lo = 0, hi = p.lines;
+    while (hi - lo > 1) {
+      const int step = (hi - lo + 31) / 32, at = lo + (lane + 1) * step;
+      const unsigned le = __ballot_sync(0xffffffffu, at < hi && p.line_at[at] <= r0);
+      lo += (__ffs(~le) - 1) * step;
+      hi = min(hi, lo + step);
+    }
+    s.places[t] = lo + t <= p.lines ? p.line_at[lo + t] : 0x7fffffff;
+    if (t == 0) s.places[128] = lo + 128 <= p.lines ? p.line_at[lo + 128] : 0x7fffffff;
+    named_bar(1, 128);
+    if (r >= first && r < end && r < p.rows) {
+      int line;
+      if (r < s.places[128]) {
+        int a = 0, b = 128;
+        while (b - a > 1) {
+          const int mid = (a + b) / 2;
+          if (s.places[mid] <= r) a = mid;
+          else b = mid;
+        }
+        line = lo + a;
+      } else {  // more than 128 lines begin in the tile (empty ones among them)
+        line = line_of_row(p.line_at, p.lines, r);
+      }
+      line = min(max(line, 0), p.lines - 1);  // (a line_at that does not ascend)
+      const int a = p.adapter ? p.adapter[line] : -1;
+      id = a >= 0 && a < p.adapters ? a : -1;
+    }
+  }
+  s.which[t] = id;
+  tile.rows[t] = make_uint4(0, 0, 0, 0);
+  named_bar(1, 128);
+  int leader = t;
+  if (id >= 0) {
+    const int4* w4 = reinterpret_cast<const int4*>(s.which);
+    for (int i = 0; i < 32; ++i) {
+      const int4 u = w4[i];
+      const int f = u.x == id ? 0 : u.y == id ? 1 : u.z == id ? 2 : u.w == id ? 3 : 4;
+      if (f < 4) {
+        leader = 4 * i + f;
+        break;
+      }
+    }
+  }
+  __syncwarp();
+  const bool leads = id >= 0 && leader == t;
+  const unsigned m = __ballot_sync(0xffffffffu, leads);
+  if (lane == 0) s.counts[q] = __popc(m);
+  named_bar(1, 128);
+  int before = 0, all = 0;
+  for (int i = 0; i < 4; ++i) {
+    before += i < q ? s.counts[i] : 0;
+    all += s.counts[i];
+  }
+  if (leads) {
+    const int k = before + __popc(m & ((1u << lane) - 1));
+    s.first_slot[t] = k;
+    tile.id[k] = id;
+  }
+  named_bar(1, 128);
+  int slot = id;
+  if (id >= 0) {
+    slot = s.first_slot[leader];
+    atomicOr(reinterpret_cast<uint32_t*>(&tile.rows[slot]) + q, 1u << lane);
+  }
+  tile.slot[t] = slot;
+  tile.scale[t] = id >= 0 ? p.scale[id] : 0.0f;
+  if (t == 0) tile.n = all;
+}
 
-// A block 16 frames x 256 classes: the frames and their adapters' inner sums in shared memory as
-// float32, a thread a class, its weights read once for the 16 frames.
-__global__ void __launch_bounds__(256) adapter_head_kernel(const __grid_constant__ AdapterParams p) {
-  __shared__ float xs[kHeadRows][kMaxHeadK];
-  __shared__ float h[kHeadRows][kMaxRank];
-  __shared__ int which[kHeadRows];  // the frame's adapter, -1 none, -2 not a line's frame
-  const int r0 = blockIdx.x * kHeadRows, n = min(kHeadRows, p.rows - r0);
-  if (threadIdx.x < kHeadRows) {
-    const int line = static_cast<int>(threadIdx.x) < n ? line_of_row(p.line_at, p.lines, r0 + threadIdx.x) : -1;
-    const int a = line < 0 || !p.adapter ? -1 : p.adapter[line];
-    which[threadIdx.x] = line < 0 ? -2 : a >= 0 && a < p.adapters ? a : -1;
-  }
-  for (int i = threadIdx.x; i < n * p.k; i += blockDim.x)
-    xs[i / p.k][i % p.k] = __half2float(p.x[(r0 + i / p.k) * p.x_pitch + i % p.k]);
-  __syncthreads();
-  for (int i = threadIdx.x; i < n * p.rank; i += blockDim.x) {
-    const int f = i / p.rank, j = i % p.rank, a = which[f];
-    float s = 0.0f;
-    if (a >= 0) {
-      const __half* row = p.a + (static_cast<long long>(a) * p.rank + j) * p.k;
-      for (int k = 0; k < p.k; ++k) s = __fmaf_rn(xs[f][k], __half2float(row[k]), s);
-      s = __fmul_rn(s, p.scale[a]);
-    }
-    h[f][j] = s;
-  }
-  __syncthreads();
-  const int c = blockIdx.y * 256 + threadIdx.x;
-  if (c >= p.classes) return;
-  float acc[kHeadRows];
-  for (int f = 0; f < kHeadRows; ++f) acc[f] = 0.0f;
-  for (int k = 0; k < p.k; ++k) {
-    const float w = __half2float(p.w[static_cast<long long>(c) * p.k + k]);
+// 16 logits of one frame (c the first's class) from their accumulators.
+__device__ __forceinline__ void store_logits(const AdapterParams& p, int r, int c, const uint32_t* acc) {
+  float v[16];
 #pragma unroll
-    for (int f = 0; f < kHeadRows; ++f) acc[f] = __fmaf_rn(xs[f][k], w, acc[f]);
+  for (int i = 0; i < 4; ++i) {
+    const float4 b = *reinterpret_cast<const float4*>(p.bias + c + 4 * i);
+    v[4 * i] = __fadd_rn(__uint_as_float(acc[4 * i]), b.x);
+    v[4 * i + 1] = __fadd_rn(__uint_as_float(acc[4 * i + 1]), b.y);
+    v[4 * i + 2] = __fadd_rn(__uint_as_float(acc[4 * i + 2]), b.z);
+    v[4 * i + 3] = __fadd_rn(__uint_as_float(acc[4 * i + 3]), b.w);
   }
-  for (int f = 0; f < n; ++f) {
-    if (which[f] == -2) continue;
-    float v = __fadd_rn(acc[f], p.bias[c]);
-    if (which[f] >= 0) {
-      const __half* row = p.b + (static_cast<long long>(which[f]) * p.classes + c) * p.rank;
-      float s = 0.0f;
-      for (int j = 0; j < p.rank; ++j) s = __fmaf_rn(h[f][j], __half2float(row[j]), s);
-      v = __fadd_rn(v, s);
+  const long long o = r * p.pitch + c;
+  const bool whole = c + 16 <= p.classes;
+  if (p.half) {
+    __half* z = static_cast<__half*>(p.z) + o;
+    if (whole && p.width >= 16) {
+      uint4 u[2];
+      uint32_t* w = reinterpret_cast<uint32_t*>(u);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+        memcpy(&w[i], &h, 4);
+      }
+      if (p.width == 32) {
+        st_global_v8(z, u[0], u[1]);
+      } else {
+        reinterpret_cast<uint4*>(z)[0] = u[0];
+        reinterpret_cast<uint4*>(z)[1] = u[1];
+      }
+      return;
     }
-    const long long o = (r0 + f) * p.pitch + c;
-    if (p.half) static_cast<__half*>(p.z)[o] = __float2half_rn(v);
-    else static_cast<float*>(p.z)[o] = v;
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (c + i < p.classes) z[i] = __float2half_rn(v[i]);
+  } else {
+    float* z = static_cast<float*>(p.z) + o;
+    if (whole && p.width >= 16) {
+      uint4 u[4];
+      memcpy(u, v, sizeof u);
+      if (p.width == 32) {
+        st_global_v8(z, u[0], u[1]);
+        st_global_v8(z + 8, u[2], u[3]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) reinterpret_cast<uint4*>(z)[i] = u[i];
+      }
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (c + i < p.classes) z[i] = v[i];
   }
+}
+
+// Persistent, an SM a block: warps 0-7 write logits (a lane a frame, the two halves of a chunk), 8-11
+// find the slots and put h back, 12 loads, 13 issues the MMAs.  An item is a tile's chunks
+// [c0, c1); its stages, in order: per slot its A rows, then per chunk W's blocks and per slot its B rows.
+__global__ void __launch_bounds__(kAdapterThreads, 1) adapter_head_kernel(const __grid_constant__ AdapterParams p) {
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* xs = smem;                                  // [nkb][128][128 bytes]
+  uint8_t* hs = xs + p.nkb * 16384;                    // h's high words, then its low words
+  uint8_t* ring = hs + 2 * p.h_bytes;                  // [stages][stage_bytes]
+  AdapterShared& s = *reinterpret_cast<AdapterShared*>(ring + p.stages * p.stage_bytes);
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kAdapterStages; ++i) {
+      mbar_init(&s.full[i], 1);
+      mbar_init(&s.empty[i], 1);
+    }
+    mbar_init(&s.a_full, 1);
+    mbar_init(&s.a_empty, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s.t_full[i], 1);
+      mbar_init(&s.t_empty[i], 8);
+      mbar_init(&s.s_full[i], 128);
+      mbar_init(&s.s_empty[i], 10);  // the loader, the MMA issuer, the eight writers
+    }
+    mbar_init(&s.h_full, 1);
+    mbar_init(&s.h2_full, 128);
+    mbar_init(&s.h2_empty, 1);
+    fence_mbar_init();
+    s.failed = 0;
+  }
+  if (warp == 13) tmem_alloc(&s.tmem, 512);
+  if (warp == 12 && lane == 0) {
+    prefetch_tmap(&p.x);
+    prefetch_tmap(&p.w);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = s.tmem, h_col = tmem + 2 * kAdapterChunk;
+  const int a_pieces = (p.nkb + p.a_stage_blocks - 1) / p.a_stage_blocks, b_pieces = (p.rank + 31) / 32;
+
+  if (warp == 12) {
+    // ---------------------------------------------------------------- loads
+    const bool leader = elect_one();
+    uint32_t g = 0;  // stages issued
+    bool ok = true;
+    auto stage = [&](uint32_t bytes) -> int {  // the next stage, empty, expecting `bytes`
+      const int i = g % p.stages;
+      ok = ok && mbar_wait_warp(&s.empty[i], ((g / p.stages) & 1) ^ 1, p.err, kErrTimeoutEmpty, p.wait_ns);
+      if (!ok) return -1;
+      ++g;
+      if (leader) mbar_expect_tx(&s.full[i], bytes);
+      __syncwarp();
+      return i;
+    };
+    uint32_t it = 0;
+    for (int item = blockIdx.x; item < p.items && ok; item += gridDim.x, ++it) {
+      const int t = item / p.splits, c0 = item % p.splits * p.chunks_per, c1 = min(p.chunks, c0 + p.chunks_per);
+      ok = mbar_wait_warp(&s.a_empty, (it & 1) ^ 1, p.err, kErrTimeoutEmpty, p.wait_ns);
+      if (!ok) break;
+      if (leader) {
+        mbar_expect_tx(&s.a_full, p.nkb * 16384);
+        for (int kb = 0; kb < p.nkb; ++kb) tma_load_3d(xs + kb * 16384, &p.x, kb * 64, t * 128, 0, &s.a_full);
+      }
+      __syncwarp();
+      ok = mbar_wait_warp(&s.s_full[it & 1], (it >> 1) & 1, p.err, kErrTimeoutFull, p.wait_ns);
+      const TileSlots& tile = s.tile[it & 1];
+      const int slots = ok ? tile.n : 0;
+      for (int k = 0; k < slots && ok; ++k)
+        for (int a = 0; a < a_pieces; ++a) {
+          const int kb0 = a * p.a_stage_blocks, kb1 = min(p.nkb, kb0 + p.a_stage_blocks);
+          const int i = stage((kb1 - kb0) * p.r16 * 128);
+          if (i < 0) break;
+          if (leader)
+            for (int kb = kb0; kb < kb1; ++kb)
+              tma_load_3d(ring + i * p.stage_bytes + (kb - kb0) * p.r16 * 128, &p.a, kb * 64, 0, tile.id[k], &s.full[i]);
+          __syncwarp();
+        }
+      for (int c = c0; c < c1 && ok; ++c) {
+        for (int kb = 0; kb < p.nkb; ++kb) {
+          const int i = stage(p.n * 128);
+          if (i < 0) break;
+          if (leader) tma_load_3d(ring + i * p.stage_bytes, &p.w, kb * 64, c * p.n, 0, &s.full[i]);
+          __syncwarp();
+        }
+        for (int k = 0; k < slots && ok; ++k)
+          for (int b = 0; b < b_pieces; ++b) {
+            const int i = stage(p.n * p.rank_row);
+            if (i < 0) break;
+            if (leader) tma_load_3d(ring + i * p.stage_bytes, &p.b, b * 32, c * p.n, tile.id[k], &s.full[i]);
+            __syncwarp();
+          }
+      }
+      if (lane == 0) mbar_arrive(&s.s_empty[it & 1]);
+    }
+    // the last tile's MMAs done (after a failure: what is on its way has arrived)
+    if (ok && it > 0) ok = mbar_wait_warp(&s.a_empty, (it & 1) ^ 1, p.err, kErrTimeoutEmpty, p.wait_ns);
+    if (!ok) {
+      mbar_wait(&s.a_full, it & 1, nullptr, 0, p.wait_ns);
+      for (uint32_t k = g > static_cast<uint32_t>(p.stages) ? g - p.stages : 0; k < g; ++k)
+        mbar_wait(&s.full[k % p.stages], (k / p.stages) & 1, nullptr, 0, p.wait_ns);
+    }
+  } else if (warp == 13) {
+    // ---------------------------------------------------------------- MMAs
+    const bool leader = elect_one();
+    const uint32_t base = __shfl_sync(0xffffffffu, tmem, 0), hbase = __shfl_sync(0xffffffffu, h_col, 0);
+    const uint32_t x0 = smem_u32(xs), ring0 = smem_u32(ring), h0 = smem_u32(hs);
+    const uint32_t id_w = idesc_f16(p.n), id_a = idesc_f16(p.r16), id_b = idesc_tf32(p.n);
+    const uint4 all_rows = make_uint4(0, 0, 0, 0);
+    uint32_t g = 0, q = 0;  // stages, accumulators taken
+    bool ok = true;
+    auto stage = [&]() -> int {
+      const int i = g % p.stages;
+      ok = ok && mbar_wait_warp(&s.full[i], (g / p.stages) & 1, p.err, kErrTimeoutFull, p.wait_ns);
+      if (!ok) return -1;
+      ++g;
+      tc_fence_after();
+      return i;
+    };
+    auto desc = [&](uint32_t addr) { return p.rank_row == 128 ? umma_desc_sw128(addr) : umma_desc_narrow(addr, p.rank_row); };
+    uint32_t it = 0, hits = 0;  // items; those with slots
+    for (int item = blockIdx.x; item < p.items && ok; item += gridDim.x, ++it) {
+      const int c0 = item % p.splits * p.chunks_per, c1 = min(p.chunks, c0 + p.chunks_per);
+      ok = mbar_wait_warp(&s.s_full[it & 1], (it >> 1) & 1, p.err, kErrTimeoutFull, p.wait_ns) &&
+           mbar_wait_warp(&s.a_full, it & 1, p.err, kErrTimeoutFull, p.wait_ns);
+      if (!ok) break;
+      tc_fence_after();
+      const TileSlots& tile = s.tile[it & 1];
+      const int slots = tile.n;
+      for (int k = 0; k < slots && ok; ++k) {
+        const uint4 on = tile.rows[k], off = make_uint4(~on.x, ~on.y, ~on.z, ~on.w);
+        for (int a = 0; a < a_pieces; ++a) {
+          const int kb0 = a * p.a_stage_blocks, kb1 = min(p.nkb, kb0 + p.a_stage_blocks);
+          const int i = stage();
+          if (i < 0) break;
+          if (leader) {
+            for (int kb = kb0; kb < kb1; ++kb) {
+              const int steps = kb == p.nkb - 1 ? p.last_steps : 4;
+              for (int u = 0; u < steps; ++u)
+                umma_rows<false>(hbase, umma_desc_sw128(x0 + kb * 16384 + u * 32),
+                                 umma_desc_sw128(ring0 + i * p.stage_bytes + (kb - kb0) * p.r16 * 128 + u * 32), id_a, off, kb | u);
+            }
+            umma_commit(&s.empty[i]);
+          }
+          __syncwarp();
+        }
+      }
+      if (slots && leader) umma_commit(&s.h_full);
+      __syncwarp();
+      for (int c = c0; c < c1 && ok; ++c, ++q) {
+        const int acc = q & 1;
+        ok = mbar_wait_warp(&s.t_empty[acc], ((q >> 1) & 1) ^ 1, p.err, kErrTimeoutTmemEmpty, p.wait_ns);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t d = base + acc * kAdapterChunk;
+        for (int kb = 0; kb < p.nkb; ++kb) {
+          const int i = stage();
+          if (i < 0) break;
+          if (leader) {
+            const int steps = kb == p.nkb - 1 ? p.last_steps : 4;
+            for (int u = 0; u < steps; ++u)
+              umma_rows<false>(d, umma_desc_sw128(x0 + kb * 16384 + u * 32), umma_desc_sw128(ring0 + i * p.stage_bytes + u * 32), id_w,
+                               all_rows, kb | u);
+            umma_commit(&s.empty[i]);
+          }
+          __syncwarp();
+        }
+        if (slots && c == c0) {
+          ok = ok && mbar_wait_warp(&s.h2_full, hits & 1, p.err, kErrTimeoutFull, p.wait_ns);
+          tc_fence_after();
+        }
+        for (int k = 0; k < slots && ok; ++k) {
+          const uint4 on = tile.rows[k], off = make_uint4(~on.x, ~on.y, ~on.z, ~on.w);
+          for (int b = 0; b < b_pieces; ++b) {
+            const int i = stage();
+            if (i < 0) break;
+            if (leader) {
+              const int steps = min(4, p.rank / 8 - 4 * b);
+              for (int u = 0; u < steps; ++u) {
+                const uint32_t at = b * 16384 + u * 32;
+                const uint64_t db = desc(ring0 + i * p.stage_bytes + u * 32);
+                umma_rows<true>(d, desc(h0 + at), db, id_b, off, 1);
+                umma_rows<true>(d, desc(h0 + p.h_bytes + at), db, id_b, off, 1);
+              }
+              umma_commit(&s.empty[i]);
+            }
+            __syncwarp();
+          }
+        }
+        if (ok && leader) umma_commit(&s.t_full[acc]);
+        __syncwarp();
+      }
+      if (!ok) break;
+      if (leader) {
+        if (slots) umma_commit(&s.h2_empty);
+        umma_commit(&s.a_empty);
+      }
+      hits += slots != 0;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s.s_empty[it & 1]);
+    }
+  } else if (warp >= 8) {
+    // ---------------------------------------------------------------- slots and h
+    const int t = threadIdx.x - 256, quarter = warp & 3;
+    const uint32_t taddr = h_col + (static_cast<uint32_t>(quarter * 32) << 16);
+    uint32_t built = 0, hits = 0, it = 0;
+    bool ok = true;
+    // the four warps' common decision: none is left waiting at a barrier of theirs
+    auto agree = [&]() {
+      if (!ok) s.failed = 1;
+      named_bar(1, 128);
+      ok = s.failed == 0;
+      named_bar(1, 128);
+      return ok;
+    };
+    auto build = [&](int item) {
+      ok = mbar_wait_warp(&s.s_empty[built & 1], ((built >> 1) & 1) ^ 1, p.err, kErrTimeoutEmpty, p.wait_ns);
+      if (!agree()) return;
+      find_slots(p, s, s.tile[built & 1], item / p.splits * 128, t);
+      mbar_arrive(&s.s_full[built & 1]);
+      ++built;
+    };
+    int item = blockIdx.x;
+    if (item < p.items) build(item);
+    for (; item < p.items && ok; item += gridDim.x, ++it) {
+      named_bar(1, 128);  // the slots are whole
+      const TileSlots& tile = s.tile[it & 1];
+      const bool more = item + static_cast<int>(gridDim.x) < p.items;
+      if (tile.n == 0) {
+        if (more) build(item + gridDim.x);
+        continue;
+      }
+      const float scale = tile.scale[t];
+      ok = mbar_wait_warp(&s.h_full, hits & 1, p.err, kErrTimeoutFull, p.wait_ns) &&
+           mbar_wait_warp(&s.h2_empty, (hits & 1) ^ 1, p.err, kErrTimeoutEmpty, p.wait_ns);
+      if (!agree()) break;
+      ++hits;
+      tc_fence_after();
+      for (int j0 = 0; j0 < p.rank; j0 += 16) {
+        uint32_t r[16];
+        tmem_ld16(taddr + j0, r);
+        tmem_wait_ld();
+        tmem_pin(r);
+#pragma unroll
+        for (int j = 0; j < 16; j += 4) {
+          if (j0 + j >= p.rank) break;
+          uint32_t hi[4], lo[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float v = __fmul_rn(__uint_as_float(r[j + i]), scale);
+            hi[i] = __float_as_uint(v) & 0xffffe000u;  // tf32: 10 bits of the fraction
+            lo[i] = __float_as_uint(__fsub_rn(v, __uint_as_float(hi[i])));
+          }
+          // 16 bytes of row t: in rows of rank_row bytes, swizzled as the MMA reads them
+          const int k = j0 + j, block = k / 32, piece = (k % 32) / 4;
+          const int swz = piece ^ ((t * p.rank_row >> 7) & (p.rank_row / 16 - 1));
+          uint8_t* at = hs + block * 16384 + t * p.rank_row + swz * 16;
+          *reinterpret_cast<uint4*>(at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+          *reinterpret_cast<uint4*>(at + p.h_bytes) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        }
+      }
+      tc_fence_before();
+      fence_proxy_async_smem();
+      mbar_arrive(&s.h2_full);
+      if (more) build(item + gridDim.x);
+    }
+  } else {
+    // ---------------------------------------------------------------- logits
+    const int quarter = warp & 3, half = warp >> 2, row = quarter * 32 + lane;
+    const int groups = p.n / 16, g0 = half ? (groups + 1) / 2 : 0, g1 = half ? groups : (groups + 1) / 2;
+    uint32_t q = 0, it = 0;
+    bool ok = true;
+    for (int item = blockIdx.x; item < p.items && ok; item += gridDim.x, ++it) {
+      const int t = item / p.splits, c0 = item % p.splits * p.chunks_per, c1 = min(p.chunks, c0 + p.chunks_per);
+      ok = mbar_wait_warp(&s.s_full[it & 1], (it >> 1) & 1, p.err, kErrTimeoutFull, p.wait_ns);
+      if (!ok) break;
+      const bool mine = s.tile[it & 1].slot[row] != -2;
+      const int r = t * 128 + row;
+      for (int c = c0; c < c1; ++c, ++q) {
+        const int acc = q & 1;
+        ok = mbar_wait_warp(&s.t_full[acc], (q >> 1) & 1, p.err, kErrTimeoutTmemFull, p.wait_ns);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t taddr = tmem + acc * kAdapterChunk + (static_cast<uint32_t>(quarter * 32) << 16);
+        for (int g = g0; g < g1; g += 2) {
+          uint32_t v[32];
+          const bool two = g + 1 < g1;
+          if (two) tmem_ld32(taddr + g * 16, v);
+          else tmem_ld16(taddr + g * 16, *reinterpret_cast<uint32_t(*)[16]>(v));
+          tmem_wait_ld();
+          tmem_pin(v);
+          const int k = c * p.n + g * 16;
+          if (mine && k < p.classes) store_logits(p, r, k, v);
+          if (mine && two && k + 16 < p.classes) store_logits(p, r, k + 16, v + 16);
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s.t_empty[acc]);
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s.s_empty[it & 1]);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 13) tmem_dealloc(tmem, 512);
 }
 
 }  // namespace crec

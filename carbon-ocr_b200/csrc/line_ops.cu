@@ -1,5 +1,6 @@
 // The C ABI's calls on the logits of packed lines (rules, greedy CTC, candidates) and the head
 // with adapters: arguments checked, parameters filled, kernels queued.
+#include <cuda.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
@@ -261,13 +262,14 @@ bool output_fits(const crec_line_logits* z, const void* out, int out_type, int64
 }  // namespace
 
 struct crec_adapters {
-  int device = 0;
-  int classes = 0, k = 0, adapters = 0, rank = 0;
-  __half* w = nullptr;
-  float* bias = nullptr;
-  __half* a = nullptr;
-  __half* b = nullptr;
+  int device = 0, sms = 0;
+  int classes = 0, k = 0, adapters = 0, rank = 0, r16 = 0;
+  __half* w = nullptr;   // [classes][k]
+  float* bias = nullptr;  // [classes], zeros to a multiple of 256
+  __half* a = nullptr;   // [adapters][r16][k]
+  float* b = nullptr;    // [adapters][classes][rank]
   float* scale = nullptr;
+  int* err = nullptr;  // pinned, written by a launch whose bounded wait ran out
 };
 
 namespace {
@@ -317,12 +319,84 @@ const char* blob_head(const uint8_t* blob, size_t bytes, int* classes, int* k, s
   return at == bytes ? nullptr : "model blob has trailing bytes";
 }
 
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                 const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiled encoder() {
+  static std::atomic<EncodeTiled> known{nullptr};
+  EncodeTiled f = known.load(std::memory_order_relaxed);
+  if (f) return f;
+  void* fn = nullptr;
+  cudaDriverEntryPointQueryResult q{};
+  if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) {
+    cudaGetLastError();
+    return nullptr;
+  }
+  f = reinterpret_cast<EncodeTiled>(fn);
+  known.store(f, std::memory_order_relaxed);
+  return f;
+}
+
+// [outer][rows][row] elements, rows `pitch` elements apart, in boxes of `box` x box_rows, the box's
+// bytes a row the swizzle's width (32, 64 or 128).
+bool encode(CUtensorMap* m, const void* base, bool half, uint64_t row, uint64_t rows, uint64_t outer, uint64_t pitch, uint32_t box,
+            uint32_t box_rows) {
+  const EncodeTiled f = encoder();
+  const uint64_t e = half ? 2 : 4;
+  const cuuint64_t dims[3] = {row, rows, outer}, strides[2] = {pitch * e, pitch * e * rows};
+  const cuuint32_t boxes[3] = {box, box_rows, 1}, steps[3] = {1, 1, 1};
+  const CUtensorMapSwizzle sw = box * e == 128  ? CU_TENSOR_MAP_SWIZZLE_128B
+                                : box * e == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                                : CU_TENSOR_MAP_SWIZZLE_32B;
+  return f && f(m, half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, const_cast<void*>(base), dims, strides,
+                boxes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, sw, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// How a head's product is cut: classes a chunk, stages of the ring, a tile's parts.
+void plan_adapters(const crec_adapters* h, AdapterParams* p) {
+  constexpr int kSmem = 232448;
+  p->nkb = (h->k + 63) / 64;
+  p->last_steps = (h->k - (p->nkb - 1) * 64 + 15) / 16;
+  p->rank = h->rank;
+  p->r16 = h->r16;
+  p->rank_row = std::min(h->rank, 32) * 4;
+  p->h_bytes = h->rank <= 32 ? 128 * p->rank_row : 2 * 16384;
+  const int tiles = (p->rows + 127) / 128;
+  const int room = kSmem - 1024 - static_cast<int>(sizeof(AdapterShared)) - p->nkb * 16384 - 2 * static_cast<int>(p->h_bytes);
+  // fewer tiles than SMs: narrower chunks, so that their parts reach every SM
+  const int want = std::max(32, (h->classes / std::max(1, h->sms / tiles) + 15) / 16 * 16);
+  for (int most = std::min(kAdapterChunk, want);; most -= 16) {
+    p->chunks = (h->classes + most - 1) / most;
+    p->n = ((h->classes + p->chunks - 1) / p->chunks + 15) / 16 * 16;
+    p->stage_bytes = std::max(p->n, p->r16) * 128;
+    p->stages = std::min(kAdapterStages, room / static_cast<int>(p->stage_bytes));
+    if (p->stages >= 4 || p->n <= p->r16 || most <= 16) break;
+  }
+  p->a_stage_blocks = std::min(p->nkb, static_cast<int>(p->stage_bytes) / (p->r16 * 128));
+  // parts: the fewest rounds of SMs times what a part takes (its chunks, and about one more for its frames)
+  long long least = 0;
+  for (int s = 1; s <= p->chunks; ++s) {
+    const int per = (p->chunks + s - 1) / s, parts = (p->chunks + per - 1) / per;
+    const long long cost = (static_cast<long long>(tiles) * parts + h->sms - 1) / h->sms * (per + 1);
+    if (s == 1 || cost < least) {
+      least = cost;
+      p->splits = parts;
+      p->chunks_per = per;
+    }
+  }
+  p->items = tiles * p->splits;
+}
+
 void free_adapters(crec_adapters* h) {
   OnDeviceOf on;
-  if (on.to(h->device) == cudaSuccess)
+  if (on.to(h->device) == cudaSuccess) {
     for (void* p : {static_cast<void*>(h->w), static_cast<void*>(h->bias), static_cast<void*>(h->a),
                     static_cast<void*>(h->b), static_cast<void*>(h->scale)})
       cudaFree(p);
+    cudaFreeHost(h->err);
+  }
   delete h;
 }
 
@@ -346,16 +420,25 @@ int open_adapters(int device, const void* model, size_t model_bytes, int n, cons
     if (ranks[i] < 1 || ranks[i] > kMaxRank) return fail(CREC_E_RANGE, "adapters_open: a rank of 1 to 64");
     rank = std::max(rank, static_cast<int>(ranks[i]));
   }
-  rank = (rank + 7) / 8 * 8;
-  // A [n][rank][k] and B [n][classes][rank], the rows past an adapter's own rank 0
-  const size_t na = static_cast<size_t>(n) * rank * k, nb = static_cast<size_t>(n) * classes * rank;
-  std::vector<uint16_t> pa(na, 0), pb(nb, 0);
+  rank = rank <= 8 ? 8 : rank <= 16 ? 16 : rank <= 32 ? 32 : 64;
+  const int r16 = std::max(16, rank);
+  // A [n][r16][k] and B [n][classes][rank], the rows past an adapter's own rank 0
+  const size_t na = static_cast<size_t>(n) * r16 * k, nb = static_cast<size_t>(n) * classes * rank;
+  std::vector<uint16_t> pa(na, 0);
+  std::vector<float> pb(nb, 0.0f);
   for (int i = 0; i < n; ++i) {
     const size_t r = static_cast<size_t>(ranks[i]);
-    std::memcpy(pa.data() + static_cast<size_t>(i) * rank * k, a, r * k * 2);
+    std::memcpy(pa.data() + static_cast<size_t>(i) * r16 * k, a, r * k * 2);
     a += r * k;
-    for (int c = 0; c < classes; ++c, b += r) std::memcpy(pb.data() + (static_cast<size_t>(i) * classes + c) * rank, b, r * 2);
+    float* o = pb.data() + static_cast<size_t>(i) * classes * rank;
+    for (int c = 0; c < classes; ++c, o += rank, b += r)
+      for (size_t j = 0; j < r; ++j) {
+        __half_raw v;
+        v.x = b[j];
+        o[j] = __half2float(__half(v));
+      }
   }
+  bias.resize((bias.size() + 255) / 256 * 256, 0.0f);
   OnDeviceOf on;
   cudaError_t e = on.to(device);
   if (e != cudaSuccess) {
@@ -371,11 +454,17 @@ int open_adapters(int device, const void* model, size_t model_bytes, int n, cons
   h->k = k;
   h->adapters = n;
   h->rank = rank;
+  h->r16 = r16;
+  if (e == cudaSuccess) e = sm_count(&h->sms);
   if (e == cudaSuccess) e = to_device(&h->w, w.data(), w.size());
   if (e == cudaSuccess) e = to_device(&h->bias, bias.data(), bias.size());
   if (e == cudaSuccess) e = to_device(&h->a, pa.data(), na);
   if (e == cudaSuccess) e = to_device(&h->b, pb.data(), nb);
   if (e == cudaSuccess) e = to_device(&h->scale, scales, static_cast<size_t>(n));
+  if (e == cudaSuccess) e = cudaHostAlloc(reinterpret_cast<void**>(&h->err), sizeof(int), cudaHostAllocMapped);
+  if (e == cudaSuccess) *h->err = 0;
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(adapter_head_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448);
   if (e != cudaSuccess) {
     cudaGetLastError();
     return fail.cuda(e, "adapters_open");
@@ -481,8 +570,13 @@ int crec_adapters_open(int device, const void* model, size_t model_bytes, int n,
 }
 
 int crec_adapters_close(crec_adapters* h) {
-  if (h) free_adapters(h);
-  return CREC_OK;
+  if (!h) return CREC_OK;
+  OnDeviceOf on;
+  cudaError_t e = on.to(h->device);
+  if (e == cudaSuccess) e = cudaDeviceSynchronize();
+  const int rc = e != cudaSuccess ? CREC_E_CUDA : *h->err ? CREC_E_TIMEOUT : CREC_OK;
+  free_adapters(h);
+  return rc;
 }
 
 int crec_adapters_logits(crec_adapters* h, const void* x, int64_t x_pitch, int64_t rows, int lines,
@@ -500,27 +594,31 @@ int crec_adapters_logits(crec_adapters* h, const void* x, int64_t x_pitch, int64
   if (!x || !line_at || !logits) return fail(CREC_E_INVALID, "adapters_logits: no x, line_at or logits");
   OnDeviceOf on;
   if (const cudaError_t e = on.to(h->device); e != cudaSuccess) return fail.cuda(e, "adapters_logits");
+  if (*static_cast<volatile int*>(h->err)) return fail(CREC_E_TIMEOUT, "adapters_logits: an earlier launch's wait ran out");
   AdapterParams p{};
-  p.x = static_cast<const __half*>(x);
-  p.x_pitch = x_pitch;
   p.rows = static_cast<int>(rows);
   p.lines = lines;
-  p.k = h->k;
   p.classes = h->classes;
   p.line_at = line_at;
-  p.adapter = adapter;
-  p.w = h->w;
-  p.bias = h->bias;
+  p.adapter = h->adapters ? adapter : nullptr;
   p.adapters = h->adapters;
-  p.rank = h->rank;
-  p.a = h->a;
-  p.b = h->b;
+  p.bias = h->bias;
   p.scale = h->scale;
   p.z = logits;
-  p.half = type == CREC_FP16;
   p.pitch = pitch;
-  const dim3 grid(static_cast<unsigned>((rows + kHeadRows - 1) / kHeadRows), static_cast<unsigned>((h->classes + 255) / 256));
-  adapter_head_kernel<<<grid, 256, 0, static_cast<cudaStream_t>(stream)>>>(p);
+  p.half = type == CREC_FP16;
+  const size_t element = type_bytes(type);
+  p.width = wide(logits, pitch, element, 32) ? 32 : wide(logits, pitch, element, 16) ? 16 : static_cast<int>(element);
+  p.err = h->err;
+  p.wait_ns = kWaitNs;
+  plan_adapters(h, &p);
+  bool maps = encode(&p.x, x, true, h->k, p.rows, 1, x_pitch, 64, 128) && encode(&p.w, h->w, true, h->k, h->classes, 1, h->k, 64, p.n);
+  if (maps && h->adapters)
+    maps = encode(&p.a, h->a, true, h->k, h->r16, h->adapters, h->k, 64, h->r16) &&
+           encode(&p.b, h->b, false, h->rank, h->classes, h->adapters, h->rank, std::min(h->rank, 32), p.n);
+  if (!maps) return fail(CREC_E_CUDA, "adapters_logits: cuTensorMapEncodeTiled failed");
+  const size_t smem = 1024 + p.nkb * 16384 + 2 * p.h_bytes + p.stages * p.stage_bytes + sizeof(AdapterShared);
+  adapter_head_kernel<<<std::min(p.items, h->sms), kAdapterThreads, smem, static_cast<cudaStream_t>(stream)>>>(p);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? CREC_OK : fail.cuda(e, "adapters_logits");
 }

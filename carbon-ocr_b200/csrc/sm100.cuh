@@ -207,6 +207,10 @@ __host__ __device__ constexpr uint32_t idesc_f16(int n) {  // A, B f16, D f32
   return (1u << 4) | (0u << 7) | (0u << 10) | (static_cast<uint32_t>(n >> 3) << 17) | ((128u >> 4) << 24);
 }
 
+__host__ __device__ constexpr uint32_t idesc_tf32(int n) {  // A, B tf32 (float32 words), D f32
+  return (1u << 4) | (2u << 7) | (2u << 10) | (static_cast<uint32_t>(n >> 3) << 17) | ((128u >> 4) << 24);
+}
+
 template <bool kInt8>
 __device__ __forceinline__ void umma(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
   if constexpr (kInt8) {
@@ -220,6 +224,25 @@ __device__ __forceinline__ void umma(uint32_t d_tmem, uint64_t a, uint64_t b, ui
         "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(
             d_tmem),
         "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+  }
+}
+
+// float32 accumulators, rows (TMEM lanes) 32 i + j left as they are where bit j of off[i] is set:
+// float16 operands (K = 16), or kTf32 (float32 words of which the top 19 bits count, K = 8).
+template <bool kTf32>
+__device__ __forceinline__ void umma_rows(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc, uint4 off, uint32_t acc) {
+  if constexpr (kTf32) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::tf32 [%0], %1, %2, %3, {%5, %6, %7, %8}, "
+        "p;\n}\n" ::"r"(d_tmem),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(off.x), "r"(off.y), "r"(off.z), "r"(off.w)
+        : "memory");
+  } else {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8}, "
+        "p;\n}\n" ::"r"(d_tmem),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(off.x), "r"(off.y), "r"(off.z), "r"(off.w)
         : "memory");
   }
 }
