@@ -27,24 +27,28 @@ constexpr int kMaxHeadK = 512;
 constexpr int kAdapterChunk = 224;  // classes: two accumulators and 64 columns of h in 512 columns of TMEM
 constexpr int kAdapterStages = 8;   // at most
 constexpr int kAdapterThreads = 14 * 32;
+constexpr int kBoxBytes = 8 * 4096;
+constexpr int kBiasPlaces = 4;  // chunks whose biases are in shared memory
 
 struct AdapterParams {
   CUtensorMap x;  // [rows][k] float16, boxes of 64 x 128 rows
   CUtensorMap w;  // [classes][k] float16, boxes of 64 x n
   CUtensorMap a;  // [adapters][r16][k] float16, boxes of 64 x r16
   CUtensorMap b;  // [adapters][classes][rank] float32, boxes of min(rank, 32) x n
+  CUtensorMap zmap;  // the logits, boxes of 128 bytes x 32 rows (where `boxes`)
   int rows, lines, classes;
   const int32_t* line_at;
   const int32_t* adapter;  // null: the head alone
   int adapters;
-  const float* bias;   // [classes], zeros to a multiple of 256
+  const float* bias;   // [classes], then 256 zeros
   const float* scale;  // [adapters]
   void* z;
   long long pitch;
   int half;
   int width;  // bytes that a row of z may be written at once: 32, 16, or an element's
+  int boxes;  // z's rows are 16-byte aligned and shared memory has room: whole boxes go out by TMA
   // tiles
-  int n, chunks, splits, chunks_per;  // classes a chunk (a multiple of 16); a tile's chunks, in `splits` parts
+  int n, chunks, splits, chunks_per;  // classes a chunk (a multiple of 128 bytes of z's); a tile's chunks, in `splits` parts
   int items;                          // tiles * splits
   int nkb, last_steps;                // 64-channel blocks of x; MMA steps (16 channels) of the last
   int rank, r16, rank_row;            // padded to 8, 16, 32 or 64; at least 16; bytes of a row of b's boxes
@@ -68,6 +72,9 @@ struct TileSlots {
 struct AdapterShared {
   uint64_t full[kAdapterStages], empty[kAdapterStages];
   uint64_t a_full, a_empty, t_full[2], t_empty[2], h_full, h2_full, h2_empty, s_full[2], s_empty[2];
+  uint64_t bias_full[kBiasPlaces], bias_empty[kBiasPlaces];
+  uint64_t pad;
+  float bias[kBiasPlaces][kAdapterChunk];
   uint32_t tmem;
   int failed;
   TileSlots tile[2];
@@ -166,11 +173,11 @@ __device__ __forceinline__ void find_slots(const AdapterParams& p, AdapterShared
 }
 
 // 16 logits of one frame (c the first's class) from their accumulators.
-__device__ __forceinline__ void store_logits(const AdapterParams& p, int r, int c, const uint32_t* acc) {
+__device__ __forceinline__ void store_logits(const AdapterParams& p, int r, int c, const uint32_t* acc, const float* bias) {
   float v[16];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const float4 b = *reinterpret_cast<const float4*>(p.bias + c + 4 * i);
+    const float4 b = *reinterpret_cast<const float4*>(bias + 4 * i);
     v[4 * i] = __fadd_rn(__uint_as_float(acc[4 * i]), b.x);
     v[4 * i + 1] = __fadd_rn(__uint_as_float(acc[4 * i + 1]), b.y);
     v[4 * i + 2] = __fadd_rn(__uint_as_float(acc[4 * i + 2]), b.z);
@@ -219,6 +226,46 @@ __device__ __forceinline__ void store_logits(const AdapterParams& p, int r, int 
   }
 }
 
+// A warp's 32 frames x 128 bytes of logits (32 of float32, 64 of float16, c the first's class) from
+// their accumulators through `box` (4 KB, in the 128-byte swizzle) out by TMA: each of its 32 rows a
+// full line of 128 bytes, where a lane's own stores would touch 32 lines an instruction.
+template <bool kHalf>
+__device__ __forceinline__ void store_box(const AdapterParams& p, uint8_t* box, uint32_t taddr, int lane, int r, int c, const float* bias) {
+  constexpr int kWords = kHalf ? 2 : 1;
+  uint4 out[8];
+#pragma unroll
+  for (int h = 0; h < kWords; ++h) {
+    uint32_t v[32];
+    tmem_ld32(taddr + 32 * h, v);
+    tmem_wait_ld();
+    tmem_pin(v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float4 b = *reinterpret_cast<const float4*>(bias + 32 * h + 4 * i);
+      const float x0 = __fadd_rn(__uint_as_float(v[4 * i]), b.x), x1 = __fadd_rn(__uint_as_float(v[4 * i + 1]), b.y);
+      const float x2 = __fadd_rn(__uint_as_float(v[4 * i + 2]), b.z), x3 = __fadd_rn(__uint_as_float(v[4 * i + 3]), b.w);
+      if constexpr (kHalf) {
+        const __half2 lo = __floats2half2_rn(x0, x1), hi = __floats2half2_rn(x2, x3);
+        uint32_t* w = reinterpret_cast<uint32_t*>(&out[4 * h + i / 2]) + 2 * (i & 1);
+        memcpy(w, &lo, 4);
+        memcpy(w + 1, &hi, 4);
+      } else {
+        out[i] = make_uint4(__float_as_uint(x0), __float_as_uint(x1), __float_as_uint(x2), __float_as_uint(x3));
+      }
+    }
+  }
+  if (lane == 0) bulk_wait_read();  // the box's last logits are on their way
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4*>(box + lane * 128 + ((i ^ (lane & 7)) << 4)) = out[i];
+  fence_proxy_async_smem();
+  __syncwarp();
+  if (lane == 0) {
+    tma_store_3d(&p.zmap, box, c, r, 0);
+    bulk_commit();
+  }
+}
+
 // Persistent, an SM a block: warps 0-7 write logits (a lane a frame, the two halves of a chunk), 8-11
 // find the slots and put h back, 12 loads, 13 issues the MMAs.  An item is a tile's chunks
 // [c0, c1); its stages, in order: per slot its A rows, then per chunk W's blocks and per slot its B rows.
@@ -227,7 +274,8 @@ __global__ void __launch_bounds__(kAdapterThreads, 1) adapter_head_kernel(const 
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* xs = smem;                                  // [nkb][128][128 bytes]
   uint8_t* hs = xs + p.nkb * 16384;                    // h's high words, then its low words
-  uint8_t* ring = hs + 2 * p.h_bytes;                  // [stages][stage_bytes]
+  uint8_t* boxes = hs + 2 * p.h_bytes;                 // [8][4096], where used
+  uint8_t* ring = boxes + (p.boxes ? kBoxBytes : 0);   // [stages][stage_bytes]
   AdapterShared& s = *reinterpret_cast<AdapterShared*>(ring + p.stages * p.stage_bytes);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   if (threadIdx.x == 0) {
@@ -242,6 +290,10 @@ __global__ void __launch_bounds__(kAdapterThreads, 1) adapter_head_kernel(const 
       mbar_init(&s.t_empty[i], 8);
       mbar_init(&s.s_full[i], 128);
       mbar_init(&s.s_empty[i], 10);  // the loader, the MMA issuer, the eight writers
+    }
+    for (int i = 0; i < kBiasPlaces; ++i) {
+      mbar_init(&s.bias_full[i], 1);
+      mbar_init(&s.bias_empty[i], 8);
     }
     mbar_init(&s.h_full, 1);
     mbar_init(&s.h2_full, 128);
@@ -263,7 +315,7 @@ __global__ void __launch_bounds__(kAdapterThreads, 1) adapter_head_kernel(const 
   if (warp == 12) {
     // ---------------------------------------------------------------- loads
     const bool leader = elect_one();
-    uint32_t g = 0;  // stages issued
+    uint32_t g = 0, q = 0;  // stages issued, chunks
     bool ok = true;
     auto stage = [&](uint32_t bytes) -> int {  // the next stage, empty, expecting `bytes`
       const int i = g % p.stages;
@@ -297,7 +349,15 @@ __global__ void __launch_bounds__(kAdapterThreads, 1) adapter_head_kernel(const 
               tma_load_3d(ring + i * p.stage_bytes + (kb - kb0) * p.r16 * 128, &p.a, kb * 64, 0, tile.id[k], &s.full[i]);
           __syncwarp();
         }
-      for (int c = c0; c < c1 && ok; ++c) {
+      for (int c = c0; c < c1 && ok; ++c, ++q) {
+        const int place = q % kBiasPlaces;
+        ok = mbar_wait_warp(&s.bias_empty[place], ((q / kBiasPlaces) & 1) ^ 1, p.err, kErrTimeoutEmpty, p.wait_ns);
+        if (!ok) break;
+        if (leader) {
+          mbar_expect_tx(&s.bias_full[place], p.n * 4);
+          bulk_load(s.bias[place], p.bias + c * p.n, p.n * 4, &s.bias_full[place]);
+        }
+        __syncwarp();
         for (int kb = 0; kb < p.nkb; ++kb) {
           const int i = stage(p.n * 128);
           if (i < 0) break;
@@ -317,6 +377,8 @@ __global__ void __launch_bounds__(kAdapterThreads, 1) adapter_head_kernel(const 
     // the last tile's MMAs done (after a failure: what is on its way has arrived)
     if (ok && it > 0) ok = mbar_wait_warp(&s.a_empty, (it & 1) ^ 1, p.err, kErrTimeoutEmpty, p.wait_ns);
     if (!ok) {
+      for (uint32_t k = q > kBiasPlaces ? q - kBiasPlaces : 0; k <= q; ++k)
+        mbar_wait(&s.bias_full[k % kBiasPlaces], (k / kBiasPlaces) & 1, nullptr, 0, p.wait_ns);
       mbar_wait(&s.a_full, it & 1, nullptr, 0, p.wait_ns);
       for (uint32_t k = g > static_cast<uint32_t>(p.stages) ? g - p.stages : 0; k < g; ++k)
         mbar_wait(&s.full[k % p.stages], (k / p.stages) & 1, nullptr, 0, p.wait_ns);
@@ -489,6 +551,7 @@ __global__ void __launch_bounds__(kAdapterThreads, 1) adapter_head_kernel(const 
     // ---------------------------------------------------------------- logits
     const int quarter = warp & 3, half = warp >> 2, row = quarter * 32 + lane;
     const int groups = p.n / 16, g0 = half ? (groups + 1) / 2 : 0, g1 = half ? groups : (groups + 1) / 2;
+    uint8_t* box = boxes + warp * 4096;
     uint32_t q = 0, it = 0;
     bool ok = true;
     for (int item = blockIdx.x; item < p.items && ok; item += gridDim.x, ++it) {
@@ -497,30 +560,47 @@ __global__ void __launch_bounds__(kAdapterThreads, 1) adapter_head_kernel(const 
       if (!ok) break;
       const bool mine = s.tile[it & 1].slot[row] != -2;
       const int r = t * 128 + row;
+      // every frame of the warp a line's (past the last, the boxes are clipped)
+      const bool whole = p.boxes && t * 128 + quarter * 32 < p.rows && __all_sync(0xffffffffu, mine || r >= p.rows);
       for (int c = c0; c < c1; ++c, ++q) {
         const int acc = q & 1;
-        ok = mbar_wait_warp(&s.t_full[acc], (q >> 1) & 1, p.err, kErrTimeoutTmemFull, p.wait_ns);
+        const int place = q % kBiasPlaces;
+        ok = mbar_wait_warp(&s.t_full[acc], (q >> 1) & 1, p.err, kErrTimeoutTmemFull, p.wait_ns) &&
+             mbar_wait_warp(&s.bias_full[place], (q / kBiasPlaces) & 1, p.err, kErrTimeoutFull, p.wait_ns);
         if (!ok) break;
+        const float* bias = s.bias[place];
         tc_fence_after();
         const uint32_t taddr = tmem + acc * kAdapterChunk + (static_cast<uint32_t>(quarter * 32) << 16);
-        for (int g = g0; g < g1; g += 2) {
-          uint32_t v[32];
-          const bool two = g + 1 < g1;
-          if (two) tmem_ld32(taddr + g * 16, v);
-          else tmem_ld16(taddr + g * 16, *reinterpret_cast<uint32_t(*)[16]>(v));
-          tmem_wait_ld();
-          tmem_pin(v);
-          const int k = c * p.n + g * 16;
-          if (mine && k < p.classes) store_logits(p, r, k, v);
-          if (mine && two && k + 16 < p.classes) store_logits(p, r, k + 16, v + 16);
+        if (whole) {  // boxes, the two halves in turn
+          const int step = p.half ? 64 : 32;
+          for (int k = half * step; k < p.n && c * p.n + k < p.classes; k += 2 * step) {
+            if (p.half) store_box<true>(p, box, taddr + k, lane, t * 128 + quarter * 32, c * p.n + k, bias + k);
+            else store_box<false>(p, box, taddr + k, lane, t * 128 + quarter * 32, c * p.n + k, bias + k);
+          }
+        } else {
+          for (int g = g0; g < g1; g += 2) {
+            uint32_t v[32];
+            const bool two = g + 1 < g1;
+            if (two) tmem_ld32(taddr + g * 16, v);
+            else tmem_ld16(taddr + g * 16, *reinterpret_cast<uint32_t(*)[16]>(v));
+            tmem_wait_ld();
+            tmem_pin(v);
+            const int k = c * p.n + g * 16;
+            if (mine && k < p.classes) store_logits(p, r, k, v, bias + g * 16);
+            if (mine && two && k + 16 < p.classes) store_logits(p, r, k + 16, v + 16, bias + g * 16 + 16);
+          }
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&s.t_empty[acc]);
+        if (lane == 0) {
+          mbar_arrive(&s.t_empty[acc]);
+          mbar_arrive(&s.bias_empty[place]);
+        }
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&s.s_empty[it & 1]);
     }
+    if (lane == 0) bulk_wait();
   }
   tc_fence_before();
   __syncthreads();

@@ -265,7 +265,7 @@ struct crec_adapters {
   int device = 0, sms = 0;
   int classes = 0, k = 0, adapters = 0, rank = 0, r16 = 0;
   __half* w = nullptr;   // [classes][k]
-  float* bias = nullptr;  // [classes], zeros to a multiple of 256
+  float* bias = nullptr;  // [classes], then 256 zeros
   __half* a = nullptr;   // [adapters][r16][k]
   float* b = nullptr;    // [adapters][classes][rank]
   float* scale = nullptr;
@@ -364,15 +364,18 @@ void plan_adapters(const crec_adapters* h, AdapterParams* p) {
   p->rank_row = std::min(h->rank, 32) * 4;
   p->h_bytes = h->rank <= 32 ? 128 * p->rank_row : 2 * 16384;
   const int tiles = (p->rows + 127) / 128;
-  const int room = kSmem - 1024 - static_cast<int>(sizeof(AdapterShared)) - p->nkb * 16384 - 2 * static_cast<int>(p->h_bytes);
+  int room = kSmem - 1024 - static_cast<int>(sizeof(AdapterShared)) - p->nkb * 16384 - 2 * static_cast<int>(p->h_bytes);
   // fewer tiles than SMs: narrower chunks, so that their parts reach every SM
-  const int want = std::max(32, (h->classes / std::max(1, h->sms / tiles) + 15) / 16 * 16);
-  for (int most = std::min(kAdapterChunk, want);; most -= 16) {
+  const int unit = p->half ? 64 : 32;  // a box's classes
+  p->boxes = p->width >= 16 && room - kBoxBytes >= 3 * 128 * std::max(unit, p->r16);
+  if (p->boxes) room -= kBoxBytes;
+  const int want = h->classes / std::max(1, h->sms / tiles);
+  for (int most = std::min(kAdapterChunk, std::max(want, unit)) / unit * unit;; most -= unit) {
     p->chunks = (h->classes + most - 1) / most;
-    p->n = ((h->classes + p->chunks - 1) / p->chunks + 15) / 16 * 16;
+    p->n = ((h->classes + p->chunks - 1) / p->chunks + unit - 1) / unit * unit;
     p->stage_bytes = std::max(p->n, p->r16) * 128;
     p->stages = std::min(kAdapterStages, room / static_cast<int>(p->stage_bytes));
-    if (p->stages >= 4 || p->n <= p->r16 || most <= 16) break;
+    if (p->stages >= 4 || p->n <= p->r16 || most <= unit) break;
   }
   p->a_stage_blocks = std::min(p->nkb, static_cast<int>(p->stage_bytes) / (p->r16 * 128));
   // parts: the fewest rounds of SMs times what a part takes (its chunks, and about one more for its frames)
@@ -438,7 +441,7 @@ int open_adapters(int device, const void* model, size_t model_bytes, int n, cons
         o[j] = __half2float(__half(v));
       }
   }
-  bias.resize((bias.size() + 255) / 256 * 256, 0.0f);
+  bias.resize(bias.size() + 256, 0.0f);  // (the last chunk's are read whole)
   OnDeviceOf on;
   cudaError_t e = on.to(device);
   if (e != cudaSuccess) {
@@ -616,8 +619,9 @@ int crec_adapters_logits(crec_adapters* h, const void* x, int64_t x_pitch, int64
   if (maps && h->adapters)
     maps = encode(&p.a, h->a, true, h->k, h->r16, h->adapters, h->k, 64, h->r16) &&
            encode(&p.b, h->b, false, h->rank, h->classes, h->adapters, h->rank, std::min(h->rank, 32), p.n);
+  if (maps && p.boxes) maps = encode(&p.zmap, logits, p.half, h->classes, p.rows, 1, pitch, p.half ? 64 : 32, 32);
   if (!maps) return fail(CREC_E_CUDA, "adapters_logits: cuTensorMapEncodeTiled failed");
-  const size_t smem = 1024 + p.nkb * 16384 + 2 * p.h_bytes + p.stages * p.stage_bytes + sizeof(AdapterShared);
+  const size_t smem = 1024 + p.nkb * 16384 + 2 * p.h_bytes + (p.boxes ? kBoxBytes : 0) + p.stages * p.stage_bytes + sizeof(AdapterShared);
   adapter_head_kernel<<<std::min(p.items, h->sms), kAdapterThreads, smem, static_cast<cudaStream_t>(stream)>>>(p);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? CREC_OK : fail.cuda(e, "adapters_logits");
