@@ -310,18 +310,22 @@ __global__ void __launch_bounds__(kAdapterThreads, 1) adapter_head_kernel(const 
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = s.tmem, h_col = tmem + 2 * kAdapterChunk;
-  const int a_pieces = (p.nkb + p.a_stage_blocks - 1) / p.a_stage_blocks, b_pieces = (p.rank + 31) / 32;
+  const int b_pieces = (p.rank + 31) / 32;
 
   if (warp == 12) {
     // ---------------------------------------------------------------- loads
     const bool leader = elect_one();
-    uint32_t g = 0, q = 0;  // stages issued, chunks
+    uint32_t g = 0, st = 0, phase = 1, q = 0;  // stages issued, the next one and its phase, chunks
     bool ok = true;
     auto stage = [&](uint32_t bytes) -> int {  // the next stage, empty, expecting `bytes`
-      const int i = g % p.stages;
-      ok = ok && mbar_wait_warp(&s.empty[i], ((g / p.stages) & 1) ^ 1, p.err, kErrTimeoutEmpty, p.wait_ns);
+      const int i = st;
+      ok = mbar_wait_warp(&s.empty[i], phase, p.err, kErrTimeoutEmpty, p.wait_ns);
       if (!ok) return -1;
       ++g;
+      if (++st == static_cast<uint32_t>(p.stages)) {
+        st = 0;
+        phase ^= 1;
+      }
       if (leader) mbar_expect_tx(&s.full[i], bytes);
       __syncwarp();
       return i;
@@ -340,8 +344,8 @@ __global__ void __launch_bounds__(kAdapterThreads, 1) adapter_head_kernel(const 
       const TileSlots& tile = s.tile[it & 1];
       const int slots = ok ? tile.n : 0;
       for (int k = 0; k < slots && ok; ++k)
-        for (int a = 0; a < a_pieces; ++a) {
-          const int kb0 = a * p.a_stage_blocks, kb1 = min(p.nkb, kb0 + p.a_stage_blocks);
+        for (int kb0 = 0, kb1; kb0 < p.nkb; kb0 = kb1) {
+          kb1 = min(p.nkb, kb0 + p.a_stage_blocks);
           const int i = stage((kb1 - kb0) * p.r16 * 128);
           if (i < 0) break;
           if (leader)
@@ -385,22 +389,34 @@ __global__ void __launch_bounds__(kAdapterThreads, 1) adapter_head_kernel(const 
     }
   } else if (warp == 13) {
     // ---------------------------------------------------------------- MMAs
+    // The whole warp runs the loop, so that descriptors and counters are warp-uniform, and one lane
+    // issues.  Descriptors differ from their operand's first only in the start address (address >> 4:
+    // a step of 32 bytes adds 2); made anew for each MMA, inside the issuing lane's branch, they took
+    // 250 cycles an MMA against the tensor cores' 80.
     const bool leader = elect_one();
-    const uint32_t base = __shfl_sync(0xffffffffu, tmem, 0), hbase = __shfl_sync(0xffffffffu, h_col, 0);
-    const uint32_t x0 = smem_u32(xs), ring0 = smem_u32(ring), h0 = smem_u32(hs);
+    const uint32_t base = __shfl_sync(0xffffffffu, tmem, 0), hbase = base + 2 * kAdapterChunk;
+    const uint32_t ring0 = smem_u32(ring), h0 = smem_u32(hs);
+    const uint64_t x_desc = umma_desc_sw128(smem_u32(xs)), w_desc = umma_desc_sw128(ring0);
+    const bool full_rows = p.rank_row == 128;
+    const uint64_t b_desc = full_rows ? w_desc : umma_desc_narrow(ring0, p.rank_row);
+    const uint64_t h_desc = full_rows ? umma_desc_sw128(h0) : umma_desc_narrow(h0, p.rank_row);
+    const uint64_t stage_step = p.stage_bytes >> 4, low = p.h_bytes >> 4, a_block = static_cast<uint32_t>(p.r16) * 8;
     const uint32_t id_w = idesc_f16(p.n), id_a = idesc_f16(p.r16), id_b = idesc_tf32(p.n);
-    const uint4 all_rows = make_uint4(0, 0, 0, 0);
-    uint32_t g = 0, q = 0;  // stages, accumulators taken
+    uint32_t st = 0, phase = 0, q = 0;  // the next stage and its phase, accumulators taken
     bool ok = true;
-    auto stage = [&]() -> int {
-      const int i = g % p.stages;
-      ok = ok && mbar_wait_warp(&s.full[i], (g / p.stages) & 1, p.err, kErrTimeoutFull, p.wait_ns);
-      if (!ok) return -1;
-      ++g;
+    auto arrive = [&]() {  // the next stage's operands
+      ok = mbar_wait_warp(&s.full[st], phase, p.err, kErrTimeoutFull, p.wait_ns);
       tc_fence_after();
-      return i;
+      return ok;
     };
-    auto desc = [&](uint32_t addr) { return p.rank_row == 128 ? umma_desc_sw128(addr) : umma_desc_narrow(addr, p.rank_row); };
+    auto release = [&]() {
+      if (leader) umma_commit(&s.empty[st]);
+      __syncwarp();
+      if (++st == static_cast<uint32_t>(p.stages)) {
+        st = 0;
+        phase ^= 1;
+      }
+    };
     uint32_t it = 0, hits = 0;  // items; those with slots
     for (int item = blockIdx.x; item < p.items && ok; item += gridDim.x, ++it) {
       const int c0 = item % p.splits * p.chunks_per, c1 = min(p.chunks, c0 + p.chunks_per);
@@ -412,22 +428,19 @@ __global__ void __launch_bounds__(kAdapterThreads, 1) adapter_head_kernel(const 
       const int slots = tile.n;
       for (int k = 0; k < slots && ok; ++k) {
         const uint4 on = tile.rows[k], off = make_uint4(~on.x, ~on.y, ~on.z, ~on.w);
-        for (int a = 0; a < a_pieces; ++a) {
-          const int kb0 = a * p.a_stage_blocks, kb1 = min(p.nkb, kb0 + p.a_stage_blocks);
-          const int i = stage();
-          if (i < 0) break;
-          if (leader) {
-            for (int kb = kb0; kb < kb1; ++kb) {
-              const int steps = kb == p.nkb - 1 ? p.last_steps : 4;
-              for (int u = 0; u < steps; ++u)
-                umma_rows<false>(hbase, umma_desc_sw128(x0 + kb * 16384 + u * 32),
-                                 umma_desc_sw128(ring0 + i * p.stage_bytes + (kb - kb0) * p.r16 * 128 + u * 32), id_a, off, kb | u);
-            }
-            umma_commit(&s.empty[i]);
+        for (int kb = 0; kb < p.nkb;) {
+          if (!arrive()) break;
+          uint64_t ad = x_desc + kb * 1024, bd = w_desc + st * stage_step;
+          for (const int kb1 = min(p.nkb, kb + p.a_stage_blocks); kb < kb1; ++kb, ad += 1024, bd += a_block) {
+            const int steps = kb == p.nkb - 1 ? p.last_steps : 4;
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+              if (u < steps && leader) umma_rows<false>(hbase, ad + 2 * u, bd + 2 * u, id_a, off, kb | u);
           }
-          __syncwarp();
+          release();
         }
       }
+      if (!ok) break;
       if (slots && leader) umma_commit(&s.h_full);
       __syncwarp();
       for (int c = c0; c < c1 && ok; ++c, ++q) {
@@ -437,37 +450,32 @@ __global__ void __launch_bounds__(kAdapterThreads, 1) adapter_head_kernel(const 
         tc_fence_after();
         const uint32_t d = base + acc * kAdapterChunk;
         for (int kb = 0; kb < p.nkb; ++kb) {
-          const int i = stage();
-          if (i < 0) break;
-          if (leader) {
-            const int steps = kb == p.nkb - 1 ? p.last_steps : 4;
-            for (int u = 0; u < steps; ++u)
-              umma_rows<false>(d, umma_desc_sw128(x0 + kb * 16384 + u * 32), umma_desc_sw128(ring0 + i * p.stage_bytes + u * 32), id_w,
-                               all_rows, kb | u);
-            umma_commit(&s.empty[i]);
-          }
-          __syncwarp();
+          if (!arrive()) break;
+          const int steps = kb == p.nkb - 1 ? p.last_steps : 4;
+          const uint64_t ad = x_desc + kb * 1024, bd = w_desc + st * stage_step;
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            if (u < steps && leader) umma<false>(d, ad + 2 * u, bd + 2 * u, id_w, kb | u);
+          release();
         }
+        if (!ok) break;
         if (slots && c == c0) {
-          ok = ok && mbar_wait_warp(&s.h2_full, hits & 1, p.err, kErrTimeoutFull, p.wait_ns);
+          ok = mbar_wait_warp(&s.h2_full, hits & 1, p.err, kErrTimeoutFull, p.wait_ns);
           tc_fence_after();
         }
         for (int k = 0; k < slots && ok; ++k) {
           const uint4 on = tile.rows[k], off = make_uint4(~on.x, ~on.y, ~on.z, ~on.w);
           for (int b = 0; b < b_pieces; ++b) {
-            const int i = stage();
-            if (i < 0) break;
-            if (leader) {
-              const int steps = min(4, p.rank / 8 - 4 * b);
-              for (int u = 0; u < steps; ++u) {
-                const uint32_t at = b * 16384 + u * 32;
-                const uint64_t db = desc(ring0 + i * p.stage_bytes + u * 32);
-                umma_rows<true>(d, desc(h0 + at), db, id_b, off, 1);
-                umma_rows<true>(d, desc(h0 + p.h_bytes + at), db, id_b, off, 1);
+            if (!arrive()) break;
+            const int steps = p.rank / 8 - 4 * b;
+            const uint64_t hd = h_desc + b * 1024, bd = b_desc + st * stage_step;
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+              if (u < steps && leader) {
+                umma_rows<true>(d, hd + 2 * u, bd + 2 * u, id_b, off, 1);
+                umma_rows<true>(d, hd + low + 2 * u, bd + 2 * u, id_b, off, 1);
               }
-              umma_commit(&s.empty[i]);
-            }
-            __syncwarp();
+            release();
           }
         }
         if (ok && leader) umma_commit(&s.t_full[acc]);
