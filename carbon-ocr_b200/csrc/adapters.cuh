@@ -6,8 +6,9 @@
 // N classes a chunk, into float32 accumulators in TMEM.  The adapters join in the same accumulators.
 // The frames of a tile may belong to many lines with many adapters; each distinct one (a slot) is a
 // few more MMAs whose output rows are masked to the slot's own (disable-output-lane), so no frame is
-// moved, and the cost goes with the distinct adapters of a tile, not its lines.  First h: every
-// slot's A rows as the B operand, all into the same columns of TMEM, a row keeping its own slot's.
+// moved, and the cost goes with the distinct adapters of a tile, not its lines.  First h: the A rows
+// of as many slots as 64 columns of TMEM hold as one B operand, each such group's product kept for its
+// slots' frames only, so that all groups share the columns; a frame reads its own slot's.
 // Four warps scale it and put it back as an A operand, as two tf32 words whose sum holds 22 bits (h
 // rounded to float16 once would cost the logits 2^-11 of the adapter's part, and its range; B's
 // float16 values are tf32 values exactly).  Then each slot's B rows over each chunk's accumulators.
@@ -31,7 +32,7 @@ constexpr int kBoxBytes = 8 * 4096;
 constexpr int kBiasPlaces = 4;  // chunks whose biases are in shared memory
 
 struct AdapterParams {
-  CUtensorMap x;  // [rows][k] float16, boxes of 64 x 128 rows
+  CUtensorMap x;  // [rows][k] float16, boxes of 64 x tile_rows
   CUtensorMap w;  // [classes][k] float16, boxes of 64 x n
   CUtensorMap a;  // [adapters][r16][k] float16, boxes of 64 x r16
   CUtensorMap b;  // [adapters][classes][rank] float32, boxes of min(rank, 32) x n
@@ -48,11 +49,12 @@ struct AdapterParams {
   int width;  // bytes that a row of z may be written at once: 32, 16, or an element's
   int boxes;  // z's rows are 16-byte aligned and shared memory has room: whole boxes go out by TMA
   // tiles
+  int tile_rows;                      // frames a tile takes of the 128 rows of an MMA
   int n, chunks, splits, chunks_per;  // classes a chunk (a multiple of 128 bytes of z's); a tile's chunks, in `splits` parts
   int items;                          // tiles * splits
   int nkb, last_steps;                // 64-channel blocks of x; MMA steps (16 channels) of the last
   int rank, r16, rank_row;            // padded to 8, 16, 32 or 64; at least 16; bytes of a row of b's boxes
-  int a_stage_blocks;                 // blocks of an adapter's A rows that a stage takes
+  int a_stage_blocks;                 // blocks of a group's A rows that a stage takes
   int stages;
   uint32_t stage_bytes, h_bytes;  // h_bytes: of one of h's two words
   int* err;
@@ -64,6 +66,7 @@ struct TileSlots {
   int n;
   int pad[3];
   uint4 rows[128];  // each slot's frames, a bit each
+  uint4 group[128];  // and each group's
   int id[128];      // and its adapter
   int slot[128];    // each frame's slot, -1 none, -2 not a line's frame
   float scale[128];
@@ -113,7 +116,7 @@ __device__ __forceinline__ void find_slots(const AdapterParams& p, AdapterShared
     s.places[t] = lo + t <= p.lines ? p.line_at[lo + t] : 0x7fffffff;
     if (t == 0) s.places[128] = lo + 128 <= p.lines ? p.line_at[lo + 128] : 0x7fffffff;
     named_bar(1, 128);
-    if (r >= first && r < end && r < p.rows) {
+    if (t < p.tile_rows && r >= first && r < end && r < p.rows) {
       int line;
       if (r < s.places[128]) {
         int a = 0, b = 128;
@@ -132,7 +135,7 @@ __device__ __forceinline__ void find_slots(const AdapterParams& p, AdapterShared
     }
   }
   s.which[t] = id;
-  tile.rows[t] = make_uint4(0, 0, 0, 0);
+  tile.rows[t] = tile.group[t] = make_uint4(0, 0, 0, 0);
   named_bar(1, 128);
   int leader = t;
   if (id >= 0) {
@@ -166,6 +169,7 @@ __device__ __forceinline__ void find_slots(const AdapterParams& p, AdapterShared
   if (id >= 0) {
     slot = s.first_slot[leader];
     atomicOr(reinterpret_cast<uint32_t*>(&tile.rows[slot]) + q, 1u << lane);
+    atomicOr(reinterpret_cast<uint32_t*>(&tile.group[slot / (64 / p.r16)]) + q, 1u << lane);
   }
   tile.slot[t] = slot;
   tile.scale[t] = id >= 0 ? p.scale[id] : 0.0f;
@@ -310,7 +314,7 @@ __global__ void __launch_bounds__(kAdapterThreads, 1) adapter_head_kernel(const 
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = s.tmem, h_col = tmem + 2 * kAdapterChunk;
-  const int b_pieces = (p.rank + 31) / 32;
+  const int b_pieces = (p.rank + 31) / 32, per_group = 64 / p.r16;
 
   if (warp == 12) {
     // ---------------------------------------------------------------- loads
@@ -336,21 +340,23 @@ __global__ void __launch_bounds__(kAdapterThreads, 1) adapter_head_kernel(const 
       ok = mbar_wait_warp(&s.a_empty, (it & 1) ^ 1, p.err, kErrTimeoutEmpty, p.wait_ns);
       if (!ok) break;
       if (leader) {
-        mbar_expect_tx(&s.a_full, p.nkb * 16384);
-        for (int kb = 0; kb < p.nkb; ++kb) tma_load_3d(xs + kb * 16384, &p.x, kb * 64, t * 128, 0, &s.a_full);
+        mbar_expect_tx(&s.a_full, p.nkb * p.tile_rows * 128);
+        for (int kb = 0; kb < p.nkb; ++kb) tma_load_3d(xs + kb * 16384, &p.x, kb * 64, t * p.tile_rows, 0, &s.a_full);
       }
       __syncwarp();
       ok = mbar_wait_warp(&s.s_full[it & 1], (it >> 1) & 1, p.err, kErrTimeoutFull, p.wait_ns);
       const TileSlots& tile = s.tile[it & 1];
       const int slots = ok ? tile.n : 0;
-      for (int k = 0; k < slots && ok; ++k)
+      for (int k = 0; k < slots && ok; k += per_group)
         for (int kb0 = 0, kb1; kb0 < p.nkb; kb0 = kb1) {
           kb1 = min(p.nkb, kb0 + p.a_stage_blocks);
-          const int i = stage((kb1 - kb0) * p.r16 * 128);
+          const int group = min(per_group, slots - k);
+          const int i = stage((kb1 - kb0) * group * p.r16 * 128);
           if (i < 0) break;
           if (leader)
             for (int kb = kb0; kb < kb1; ++kb)
-              tma_load_3d(ring + i * p.stage_bytes + (kb - kb0) * p.r16 * 128, &p.a, kb * 64, 0, tile.id[k], &s.full[i]);
+              for (int j = 0; j < group; ++j)
+                tma_load_3d(ring + i * p.stage_bytes + (kb - kb0) * 8192 + j * p.r16 * 128, &p.a, kb * 64, 0, tile.id[k + j], &s.full[i]);
           __syncwarp();
         }
       for (int c = c0; c < c1 && ok; ++c, ++q) {
@@ -400,8 +406,8 @@ __global__ void __launch_bounds__(kAdapterThreads, 1) adapter_head_kernel(const 
     const bool full_rows = p.rank_row == 128;
     const uint64_t b_desc = full_rows ? w_desc : umma_desc_narrow(ring0, p.rank_row);
     const uint64_t h_desc = full_rows ? umma_desc_sw128(h0) : umma_desc_narrow(h0, p.rank_row);
-    const uint64_t stage_step = p.stage_bytes >> 4, low = p.h_bytes >> 4, a_block = static_cast<uint32_t>(p.r16) * 8;
-    const uint32_t id_w = idesc_f16(p.n), id_a = idesc_f16(p.r16), id_b = idesc_tf32(p.n);
+    const uint64_t stage_step = p.stage_bytes >> 4, low = p.h_bytes >> 4, a_block = 8192 >> 4;
+    const uint32_t id_w = idesc_f16(p.n), id_b = idesc_tf32(p.n);
     uint32_t st = 0, phase = 0, q = 0;  // the next stage and its phase, accumulators taken
     bool ok = true;
     auto arrive = [&]() {  // the next stage's operands
@@ -426,8 +432,9 @@ __global__ void __launch_bounds__(kAdapterThreads, 1) adapter_head_kernel(const 
       tc_fence_after();
       const TileSlots& tile = s.tile[it & 1];
       const int slots = tile.n;
-      for (int k = 0; k < slots && ok; ++k) {
-        const uint4 on = tile.rows[k], off = make_uint4(~on.x, ~on.y, ~on.z, ~on.w);
+      for (int k = 0; k < slots && ok; k += per_group) {
+        const uint4 on = tile.group[k / per_group], off = make_uint4(~on.x, ~on.y, ~on.z, ~on.w);
+        const uint32_t id_a = idesc_f16(min(per_group, slots - k) * p.r16);
         for (int kb = 0; kb < p.nkb;) {
           if (!arrive()) break;
           uint64_t ad = x_desc + kb * 1024, bd = w_desc + st * stage_step;
@@ -507,7 +514,7 @@ __global__ void __launch_bounds__(kAdapterThreads, 1) adapter_head_kernel(const 
     auto build = [&](int item) {
       ok = mbar_wait_warp(&s.s_empty[built & 1], ((built >> 1) & 1) ^ 1, p.err, kErrTimeoutEmpty, p.wait_ns);
       if (!agree()) return;
-      find_slots(p, s, s.tile[built & 1], item / p.splits * 128, t);
+      find_slots(p, s, s.tile[built & 1], item / p.splits * p.tile_rows, t);
       mbar_arrive(&s.s_full[built & 1]);
       ++built;
     };
@@ -522,6 +529,7 @@ __global__ void __launch_bounds__(kAdapterThreads, 1) adapter_head_kernel(const 
         continue;
       }
       const float scale = tile.scale[t];
+      const int place = max(tile.slot[t], 0) % per_group * p.r16;  // this frame's columns of h
       ok = mbar_wait_warp(&s.h_full, hits & 1, p.err, kErrTimeoutFull, p.wait_ns) &&
            mbar_wait_warp(&s.h2_empty, (hits & 1) ^ 1, p.err, kErrTimeoutEmpty, p.wait_ns);
       if (!agree()) break;
@@ -529,9 +537,15 @@ __global__ void __launch_bounds__(kAdapterThreads, 1) adapter_head_kernel(const 
       tc_fence_after();
       for (int j0 = 0; j0 < p.rank; j0 += 16) {
         uint32_t r[16];
-        tmem_ld16(taddr + j0, r);
-        tmem_wait_ld();
-        tmem_pin(r);
+        for (int g = 0; g < 64; g += p.r16) {  // every slot's place, a lane keeping its own
+          if (!__any_sync(0xffffffffu, place == g)) continue;
+          uint32_t u[16];
+          tmem_ld16(taddr + g + j0, u);
+          tmem_wait_ld();
+          tmem_pin(u);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) r[i] = place == g ? u[i] : r[i];
+        }
 #pragma unroll
         for (int j = 0; j < 16; j += 4) {
           if (j0 + j >= p.rank) break;
@@ -567,9 +581,9 @@ __global__ void __launch_bounds__(kAdapterThreads, 1) adapter_head_kernel(const 
       ok = mbar_wait_warp(&s.s_full[it & 1], (it >> 1) & 1, p.err, kErrTimeoutFull, p.wait_ns);
       if (!ok) break;
       const bool mine = s.tile[it & 1].slot[row] != -2;
-      const int r = t * 128 + row;
+      const int r = t * p.tile_rows + row;
       // every frame of the warp a line's (past the last, the boxes are clipped)
-      const bool whole = p.boxes && t * 128 + quarter * 32 < p.rows && __all_sync(0xffffffffu, mine || r >= p.rows);
+      const bool whole = p.boxes && t * p.tile_rows + quarter * 32 < p.rows && __all_sync(0xffffffffu, mine || r >= p.rows);
       for (int c = c0; c < c1; ++c, ++q) {
         const int acc = q & 1;
         const int place = q % kBiasPlaces;
@@ -582,8 +596,8 @@ __global__ void __launch_bounds__(kAdapterThreads, 1) adapter_head_kernel(const 
         if (whole) {  // boxes, the two halves in turn
           const int step = p.half ? 64 : 32;
           for (int k = half * step; k < p.n && c * p.n + k < p.classes; k += 2 * step) {
-            if (p.half) store_box<true>(p, box, taddr + k, lane, t * 128 + quarter * 32, c * p.n + k, bias + k);
-            else store_box<false>(p, box, taddr + k, lane, t * 128 + quarter * 32, c * p.n + k, bias + k);
+            if (p.half) store_box<true>(p, box, taddr + k, lane, t * p.tile_rows + quarter * 32, c * p.n + k, bias + k);
+            else store_box<false>(p, box, taddr + k, lane, t * p.tile_rows + quarter * 32, c * p.n + k, bias + k);
           }
         } else {
           for (int g = g0; g < g1; g += 2) {

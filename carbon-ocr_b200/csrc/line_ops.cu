@@ -354,7 +354,7 @@ bool encode(CUtensorMap* m, const void* base, bool half, uint64_t row, uint64_t 
                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// How a head's product is cut: classes a chunk, stages of the ring, a tile's parts.
+// How a head's product is cut: frames a tile, classes a chunk, stages of the ring, a tile's parts.
 void plan_adapters(const crec_adapters* h, AdapterParams* p) {
   constexpr int kSmem = 232448;
   p->nkb = (h->k + 63) / 64;
@@ -363,33 +363,47 @@ void plan_adapters(const crec_adapters* h, AdapterParams* p) {
   p->r16 = h->r16;
   p->rank_row = std::min(h->rank, 32) * 4;
   p->h_bytes = h->rank <= 32 ? 128 * p->rank_row : 2 * 16384;
-  const int tiles = (p->rows + 127) / 128;
   int room = kSmem - 1024 - static_cast<int>(sizeof(AdapterShared)) - p->nkb * 16384 - 2 * static_cast<int>(p->h_bytes);
-  // fewer tiles than SMs: narrower chunks, so that their parts reach every SM
   const int unit = p->half ? 64 : 32;  // a box's classes
-  p->boxes = p->width >= 16 && room - kBoxBytes >= 3 * 128 * std::max(unit, p->r16);
+  p->boxes = p->width >= 16 && room - kBoxBytes >= 3 * 8192;
   if (p->boxes) room -= kBoxBytes;
-  const int want = h->classes / std::max(1, h->sms / tiles);
-  for (int most = std::min(kAdapterChunk, std::max(want, unit)) / unit * unit;; most -= unit) {
-    p->chunks = (h->classes + most - 1) / most;
-    p->n = ((h->classes + p->chunks - 1) / p->chunks + unit - 1) / unit * unit;
-    p->stage_bytes = std::max(p->n, p->r16) * 128;
-    p->stages = std::min(kAdapterStages, room / static_cast<int>(p->stage_bytes));
-    if (p->stages >= 4 || p->n <= p->r16 || most <= unit) break;
-  }
-  p->a_stage_blocks = std::min(p->nkb, static_cast<int>(p->stage_bytes) / (p->r16 * 128));
-  // parts: the fewest rounds of SMs times what a part takes (its chunks, and about one more for its frames)
-  long long least = 0;
-  for (int s = 1; s <= p->chunks; ++s) {
-    const int per = (p->chunks + s - 1) / s, parts = (p->chunks + per - 1) / per;
-    const long long cost = (static_cast<long long>(tiles) * parts + h->sms - 1) / h->sms * (per + 1);
-    if (s == 1 || cost < least) {
-      least = cost;
-      p->splits = parts;
-      p->chunks_per = per;
+  // Of tiles of 128 frames or fewer, chunks of kAdapterChunk classes or fewer and a tile's chunks in one
+  // part or as many as reach every SM, the cheapest: rounds of SMs times what a part takes, in 0.1 us as
+  // measured (K = 256, 160 classes a chunk): 4 us for its frames and h, 0.4 us a block of 64 channels a
+  // chunk, 0.5 us an adapter a chunk, and not less than its logits take at an SM's share of HBM.  Fewer
+  // frames a tile mean fewer adapters in it, whose MMAs come one after another.
+  double least = 0;
+  for (int rows = 128; rows >= 16; rows /= 2) {
+    const int tiles = (p->rows + rows - 1) / rows;
+    const double lines = std::min<double>(rows, 1.0 + static_cast<double>(p->lines) * rows / p->rows);  // that a tile meets
+    const double slots = p->adapter ? std::min<double>(lines, h->adapters) : 0.0;
+    for (const int wide : {224, 160, 96, 64, 32}) {
+      const int most = std::max(unit, wide / unit * unit), chunks = (h->classes + most - 1) / most;
+      const int n = ((h->classes + chunks - 1) / chunks + unit - 1) / unit * unit;
+      const int stage = std::max(n * 128, 8192), stages = std::min(kAdapterStages, room / stage);
+      if (stages < 2 || (stages < 3 && n > unit)) continue;
+      const double chunk = std::max(p->nkb * (2.0 + n / 80.0) + slots * (2.0 + n / 60.0) * ((p->rank + 15) / 16),
+                                    static_cast<double>(rows) * n * (p->half ? 2 : 4) / 4300.0);
+      const int most_parts = std::min(chunks, std::max(1, h->sms / tiles));
+      for (const int s : {1, 2, most_parts}) {
+        if (s > chunks) continue;
+        const int per = (chunks + s - 1) / s, parts = (chunks + per - 1) / per;
+        const long long rounds = (static_cast<long long>(tiles) * parts + h->sms - 1) / h->sms;
+        const double cost = rounds * (40.0 + slots * p->nkb * 0.5 + per * chunk);
+        if (least != 0 && cost >= least) continue;
+        least = cost;
+        p->tile_rows = rows;
+        p->chunks = chunks;
+        p->n = n;
+        p->stage_bytes = stage;
+        p->stages = stages;
+        p->splits = parts;
+        p->chunks_per = per;
+        p->items = tiles * parts;
+      }
     }
   }
-  p->items = tiles * p->splits;
+  p->a_stage_blocks = std::min(p->nkb, static_cast<int>(p->stage_bytes) / 8192);
 }
 
 void free_adapters(crec_adapters* h) {
@@ -615,7 +629,7 @@ int crec_adapters_logits(crec_adapters* h, const void* x, int64_t x_pitch, int64
   p.err = h->err;
   p.wait_ns = kWaitNs;
   plan_adapters(h, &p);
-  bool maps = encode(&p.x, x, true, h->k, p.rows, 1, x_pitch, 64, 128) && encode(&p.w, h->w, true, h->k, h->classes, 1, h->k, 64, p.n);
+  bool maps = encode(&p.x, x, true, h->k, p.rows, 1, x_pitch, 64, p.tile_rows) && encode(&p.w, h->w, true, h->k, h->classes, 1, h->k, 64, p.n);
   if (maps && h->adapters)
     maps = encode(&p.a, h->a, true, h->k, h->r16, h->adapters, h->k, 64, h->r16) &&
            encode(&p.b, h->b, false, h->rank, h->classes, h->adapters, h->rank, std::min(h->rank, 32), p.n);
