@@ -144,22 +144,21 @@ cudaError_t launch_on(K* k, const LineParams& p, long long blocks, int threads, 
   return cudaGetLastError();
 }
 
-// Blocks that an SM holds at once (227 KB of shared memory, 1 KB of it each block's own; 64 K registers).
-int blocks_an_sm(size_t smem, int warps, int registers) {
-  return std::max(1, std::min(static_cast<int>((228 << 10) / (smem + 1024)), 65536 / (registers * 32 * warps)));
+// Blocks that an SM holds at once: 228 KB of shared memory, 1 KB of it each block's own, and as many
+// warps as the kernel's registers leave.
+int blocks_an_sm(size_t smem, int warps, int most_warps) {
+  return std::max(1, std::min(static_cast<int>((228 << 10) / (smem + 1024)), most_warps / warps));
 }
 
 // The launches with NV vectors of V classes a lane, NV the fewest in a list that hold `classes` in a
 // team's registers.
-constexpr int kAloneWarps = 2;  // of a block whose warps take rows alone
-
 template <int kOp, typename T, int V, int NV, bool kTeam>
 cudaError_t decode_rows(LineParams& p, int sms, cudaStream_t s) {
-  using Row = WarpRow<T, V, NV>;
-  constexpr size_t kTeamRow = kTeam || kOp == kOpCandidates ? sizeof(TeamRow) : 0;
+  using Row = WarpRow<T, V, NV, kDecodeEntries>;
+  constexpr size_t kTeamRow = kTeam || kOp == kOpCandidates || Row::kSpan > Row::kCap ? sizeof(TeamRow) : 0;
   const int warps = kTeam ? p.warps : kAloneWarps, teams = kTeam ? 1 : warps;
   const size_t smem = teams * kTeamRow + static_cast<size_t>(warps) * Row::kShared;
-  const long long resident = blocks_an_sm(smem, warps, 128) * static_cast<long long>(teams) * sms;
+  const long long resident = blocks_an_sm(smem, warps, kDecodeWarps) * static_cast<long long>(teams) * sms;
   p.team_rows = static_cast<int>(std::max(1ll, (p.rows + resident - 1) / resident));
   const long long per_block = static_cast<long long>(p.team_rows) * teams;
   return launch_on(line_rows_kernel<kOp, T, V, NV, kTeam>, p, (p.rows + per_block - 1) / per_block, warps * 32, smem, s);
@@ -191,16 +190,17 @@ cudaError_t decode(LineParams& p, cudaStream_t s) {
 
 template <int kOp, typename T>
 cudaError_t decode_wide(LineParams& p, cudaStream_t s) {
-  return launch_on(wide_rows_kernel<kOp, T>, p, p.rows, 32 * kMaxTeam, sizeof(TeamRow) + static_cast<size_t>(kMaxTeam) * kWideSpan * 10, s);
+  return launch_on(wide_rows_kernel<kOp, T>, p, p.rows, 32 * kMaxTeam,
+                   sizeof(TeamRow) + static_cast<size_t>(kMaxTeam) * SpanRules<kSlowSpan, kSlowSpan>::kBytes, s);
 }
 
 template <typename T, typename O, int V, int NV>
 cudaError_t write_rows(LineParams& p, int sms, cudaStream_t s) {
-  using Row = WarpRow<T, V, NV>;
+  using Row = WarpRow<T, V, NV, 32 * V * NV>;
   constexpr int kWarps = kRulesThreads / 32;
   p.chunks = (p.classes + Row::kSpan - 1) / Row::kSpan;
   const size_t smem = static_cast<size_t>(kWarps) * Row::kShared;
-  const long long resident = blocks_an_sm(smem, kWarps, 64) * static_cast<long long>(kWarps) * sms;
+  const long long resident = blocks_an_sm(smem, kWarps, 32) * static_cast<long long>(kWarps) * sms;
   p.team_rows = static_cast<int>(std::max(1ll, (static_cast<long long>(p.rows) * p.chunks + resident - 1) / resident));
   const long long units = (p.rows + p.team_rows - 1) / p.team_rows * static_cast<long long>(p.chunks);
   return launch_on(logit_rules_kernel<T, O, V, NV>, p, (units + kWarps - 1) / kWarps, kRulesThreads, smem, s);
@@ -232,7 +232,6 @@ cudaError_t launch_decode(LineParams& p, int type, cudaStream_t s) {
 
 cudaError_t launch_rules(LineParams& p, int type, int out_type, cudaStream_t s) {
   bias_reads(p);
-  p.in_place = p.z == p.out;
   const bool w = wide(p.z, p.pitch, type_bytes(type), 16);
   if (type == CREC_FP16) {
     if (out_type == CREC_FP16)
@@ -530,8 +529,17 @@ int crec_ctc_greedy_lines(const crec_line_logits* z, const crec_rules* rules, in
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t e = p.rows > 0 ? launch_decode<kOpGreedy>(p, z->type, s) : cudaSuccess;
   if (e == cudaSuccess) {
-    collapse_lines_kernel<<<(p.lines + 3) / 4, 128, 0, s>>>(p);
-    e = cudaGetLastError();
+    // queued to start while the frames' last blocks run
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(static_cast<unsigned>((p.lines + 3) / 4));
+    config.blockDim = dim3(128);
+    config.stream = s;
+    cudaLaunchAttribute early{};
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = p.rows > 0;
+    config.attrs = &early;
+    config.numAttrs = 1;
+    e = cudaLaunchKernelEx(&config, collapse_lines_kernel, p);
   }
   return e == cudaSuccess ? CREC_OK : fail.cuda(e, "ctc_greedy_lines");
 }

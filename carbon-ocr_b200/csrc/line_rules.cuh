@@ -44,7 +44,6 @@ struct LineParams {
   int warps;      // of a team, a power of two
   int chunks;     // rules: the spans that a row takes
   int team_rows;  // rows a team takes
-  int in_place;   // the ruled logits go where the logits are
   int bias_wide;  // the bias tables' rows may be read 16 bytes at a time
 };
 
@@ -122,6 +121,7 @@ __device__ __forceinline__ unsigned long long class_key(float v, int c) {
 // a row is worked on.
 
 constexpr int kDecodeLane = 32;  // classes a lane holds in the decoders: 128 registers, 16 warps an SM
+constexpr int kDecodeEntries = 256;  // of a span in the decoders; a line with more goes the slow way
 constexpr int kRulesLane = 16;   // and where the ruled logits are written
 constexpr int kMaxTeam = 16;     // warps that share a row
 constexpr int kMaxClasses = 65536;
@@ -171,10 +171,10 @@ __device__ __forceinline__ void get_logits(const __half* z, float* v) {
   }
 }
 
-// V ruled logits written at o, those in `gone` (a bit each) left to the list.
+// V ruled logits (n of them classes) written at o.
 template <typename O, int V>
-__device__ __forceinline__ void store_ruled(O* o, const float* v, uint32_t gone, int n) {
-  if (V > 1 && gone == 0 && n >= V) {
+__device__ __forceinline__ void store_ruled(O* o, const float* v, int n) {
+  if (V > 1 && n >= V) {
     if constexpr (sizeof(O) == 2) {
       uint32_t w[V / 2 > 0 ? V / 2 : 1];
 #pragma unroll
@@ -193,11 +193,16 @@ __device__ __forceinline__ void store_ruled(O* o, const float* v, uint32_t gone,
   }
 #pragma unroll
   for (int i = 0; i < V; ++i)
-    if (i < n && !(gone >> i & 1)) {
+    if (i < n) {
       if constexpr (sizeof(O) == 2) o[i] = __float2half_rn(v[i]);
       else o[i] = v[i];
     }
 }
+
+// Programmatic dependent launch: a kernel queued to start early waits here for the one before it to
+// be done; that one says, once all its blocks run, that the next may start.
+__device__ __forceinline__ void launch_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void launch_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 __device__ __forceinline__ float warp_max(float v) {
   float m;
@@ -228,11 +233,11 @@ __device__ __forceinline__ float exp_less(float v, float c) { return ex2_approx(
 // A row's best (0 where nothing is left) and what its sums are taken against.
 struct RowBase {
   float best, c;
-  bool fits;  // c is finite; else (|best| past 2.3e38) the difference is taken first
+  bool fits;  // c's rounding is below 2^-4; else (|best| past 7e5) the difference is taken first
   __device__ __forceinline__ explicit RowBase(float b) {
     best = b == -INFINITY ? 0.0f : b;
     c = __fmul_rn(best, kLog2e);
-    fits = fabsf(c) < INFINITY;
+    fits = fabsf(c) < 1048576.0f;
   }
   __device__ __forceinline__ float term(float v) const { return fits ? exp_less(v, c) : ex2_approx(__fmul_rn(__fsub_rn(v, best), kLog2e)); }
 };
@@ -247,26 +252,31 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   return d;
 }
 
-// A warp's part of shared memory: 10 bytes a class of its span.  add: what the rules add to each class
-// in the dense pass, -inf for what the set leaves out, for the history's classes and past the last
-// class; while a line's rules are set, the history's counts.  Then the entries: the history's classes
-// that are allowed, places within the span and n * frequency + presence.
+// A warp's part of shared memory: add, what the rules add to each class of its span in the dense pass,
+// -inf for what the set leaves out, for the history's classes and past the last class (while a
+// line's rules are set, the history's counts); then the entries, the history's classes that are
+// allowed: n * frequency + presence, and places within the span; at most kCap are kept.
+template <int kSpan, int kCap>
 struct SpanRules {
   float* add;
   float* less;
   uint16_t* at;
-  __device__ __forceinline__ SpanRules(uint8_t* shared, int span)
-      : add(reinterpret_cast<float*>(shared)), less(add + span), at(reinterpret_cast<uint16_t*>(less + span)) {}
+  __device__ __forceinline__ explicit SpanRules(uint8_t* shared) {
+    add = reinterpret_cast<float*>(shared);
+    less = add + kSpan;
+    at = reinterpret_cast<uint16_t*>(less + kCap);
+  }
+  static constexpr int kBytes = kSpan * 4 + kCap * 6;
 };
 
 // A line's rules on the classes [base, base + 32 * V * NV) into a warp's SpanRules; the number of
-// entries.  *gone (rules written out only): bit j * V + i, this lane's class base + (j * 32 + lane) * V + i
-// is an entry.  Once a line: not inlined, its code out of the rows' way.
-template <int V, int NV>
+// entries (past kCap they are counted, not kept).  Once a line: not inlined, its code out of the
+// rows' way.
+template <int V, int NV, int kCap>
 __device__ __noinline__ int set_rules(uint8_t* shared, int classes, int base, const int32_t* had, int n_had, float presence,
-                                      float frequency, const float* bias, bool bias_wide, const uint32_t* allowed, uint32_t* gone) {
+                                      float frequency, const float* bias, bool bias_wide, const uint32_t* allowed) {
   constexpr int kSpan = 32 * V * NV;
-  const SpanRules s(shared, kSpan);
+  const SpanRules<kSpan, kCap> s(shared);
   const int lane = threadIdx.x % 32;
   uint32_t* count = reinterpret_cast<uint32_t*>(s.add);
   int n = 0;
@@ -279,9 +289,23 @@ __device__ __noinline__ int set_rules(uint8_t* shared, int classes, int base, co
       if (c >= 0 && c < kSpan) atomicAdd(&count[c], 1u);
     }
     __syncwarp();
+    // each class once: whoever takes its count makes the entry
+    for (int k0 = 0; k0 < n_had; k0 += 32) {
+      const int c = k0 + lane < n_had ? had[k0 + lane] - base : -1;
+      const uint32_t times = c >= 0 && c < kSpan ? atomicExch(&count[c], 0u) : 0u;
+      const bool left_out = times && (base + c >= classes || (allowed && !(allowed[(base + c) >> 5] >> ((base + c) & 31) & 1)) ||
+                                      (bias && bias[base + c] == -INFINITY));
+      const unsigned m = __ballot_sync(0xffffffffu, times && !left_out);
+      const int e = n + __popc(m & ((1u << lane) - 1));
+      if ((m >> lane & 1) && e < kCap) {
+        s.at[e] = static_cast<uint16_t>(c);
+        s.less[e] = __fadd_rn(__fmul_rn(static_cast<float>(times), frequency), presence);
+      }
+      n += __popc(m);
+    }
+    __syncwarp();
   }
-  uint32_t mine = 0;
-#pragma unroll 1
+#pragma unroll
   for (int j = 0; j < NV; ++j) {
     const int k = (j * 32 + lane) * V, c = base + k;
     const uint32_t keep = allowed && c < classes ? allowed[c >> 5] >> (c & 31) : ~0u;
@@ -300,28 +324,11 @@ __device__ __noinline__ int set_rules(uint8_t* shared, int classes, int base, co
       for (int i = 0; i < V; ++i) b[i] = bias && c + i < classes ? bias[c + i] : 0.0f;
     }
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const uint32_t times = n_had > 0 ? count[k + i] : 0u;
-      const bool in = c + i < classes && (keep >> i & 1);
-      if (n_had > 0) {
-        const bool entry = times != 0 && in && b[i] != -INFINITY;
-        const unsigned m = __ballot_sync(0xffffffffu, entry);
-        if (entry) {
-          const int e = n + __popc(m & ((1u << lane) - 1));
-          s.at[e] = static_cast<uint16_t>(k + i);
-          s.less[e] = __fadd_rn(__fmul_rn(static_cast<float>(times), frequency), presence);
-          mine |= 1u << (j * V + i);
-        }
-        n += __popc(m);
-      }
-      b[i] = in && times == 0 ? b[i] : -INFINITY;
-    }
-    // a vector of the table is its lane's own: the counts that others have yet to read stay
-#pragma unroll
-    for (int i = 0; i < V; ++i) s.add[k + i] = b[i];
+    for (int i = 0; i < V; ++i) s.add[k + i] = c + i < classes && (keep >> i & 1) ? b[i] : -INFINITY;
   }
   __syncwarp();
-  if (gone) *gone = mine;
+  for (int e = lane; e < min(n, kCap); e += 32) s.add[s.at[e]] = -INFINITY;
+  __syncwarp();
   return n;
 }
 
@@ -335,10 +342,12 @@ __device__ __noinline__ float far_entry(const T* z, const float* less, const uin
 
 // A warp's span of a row, and its line's rules on it.  Rows come through a place in shared memory:
 // while one is worked on, in registers, the next is on its way there.
-template <typename T, int V, int NV>
+template <typename T, int V, int NV, int kMaxEntries>
 struct WarpRow {
   static constexpr int kLane = NV * V, kSpan = 32 * kLane;  // classes of a lane, of the warp
-  static constexpr int kShared = kSpan * (10 + sizeof(T));
+  static constexpr int kCap = kSpan < kMaxEntries ? kSpan : kMaxEntries;
+  using Rules = SpanRules<kSpan, kCap>;
+  static constexpr int kRules = Rules::kBytes, kShared = kRules + kSpan * sizeof(T);
   int lane, base;  // the span's first class
   LineRule l;
   uint8_t* shared;  // SpanRules, then the rows
@@ -360,7 +369,7 @@ struct WarpRow {
   __device__ __forceinline__ const T* row(const LineParams& p, int r) const {
     return static_cast<const T*>(p.z) + r * p.pitch + base;
   }
-  __device__ __forceinline__ T* place() const { return reinterpret_cast<T*>(shared + kSpan * 10); }
+  __device__ __forceinline__ T* place() const { return reinterpret_cast<T*>(shared + kRules); }
   // Row r (where r < r1) on its way.
   __device__ __forceinline__ void fetch(const LineParams& p, int r, int r1) {
     if (r < r1) {
@@ -384,9 +393,9 @@ struct WarpRow {
     __syncwarp();
   }
   // The rules of the line that the row lies in.
-  __device__ __forceinline__ void rules(const LineParams& p, uint32_t* gone) {
-    n = set_rules<V, NV>(shared, p.classes, base, l.had, l.n_had, l.presence, l.frequency, l.bias, p.bias_wide, l.allowed, gone);
-    const SpanRules s(shared, kSpan);
+  __device__ __forceinline__ void rules(const LineParams& p) {
+    n = set_rules<V, NV, kCap>(shared, p.classes, base, l.had, l.n_had, l.presence, l.frequency, l.bias, p.bias_wide, l.allowed);
+    const Rules s(shared);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       if (lane + 32 * i >= n) continue;
@@ -441,17 +450,17 @@ struct WarpRow {
     for (int i = 0; i < 2; ++i)
       if (lane + 32 * i < n) x[i] = __fadd_rn(penalised(load_logit(place() + at[i]), less[i], l.repeat), plus[i]);
   }
-  // f(ruled logit, class) for each of this lane's entries in row r, x the first.
+  // f(ruled logit, class) for each of this lane's entries in the row at z, x the first.
   template <typename F>
-  __device__ __forceinline__ void entries(const LineParams& p, int r, const float (&x)[2], F f) const {
+  __device__ __forceinline__ void entries(const T* z, const float (&x)[2], F f) const {
     if (n == 0) return;
 #pragma unroll
     for (int i = 0; i < 2; ++i)
       if (lane + 32 * i < n) f(x[i], base + at[i]);
     if (n <= 64) return;
-    const SpanRules s(shared, kSpan);
+    const Rules s(shared);
 #pragma unroll 1
-    for (int e = lane + 64; e < n; e += 32) f(far_entry(row(p, r), s.less, s.at, e, l.repeat, l.bias, base), base + s.at[e]);
+    for (int e = lane + 64; e < n; e += 32) f(far_entry(z, s.less, s.at, e, l.repeat, l.bias, base), base + s.at[e]);
   }
 };
 
@@ -468,16 +477,15 @@ __global__ void __launch_bounds__(kRulesThreads, 8) logit_rules_kernel(const __g
   const long long r0 = unit / p.chunks * p.team_rows;
   const int r1 = static_cast<int>(min(static_cast<long long>(p.rows), r0 + p.team_rows));
   if (r0 >= r1) return;
-  using Row = WarpRow<T, V, NV>;
+  using Row = WarpRow<T, V, NV, 32 * V * NV>;  // every class may be an entry
   Row row;
   row.start(p, static_cast<int>(unit % p.chunks) * Row::kSpan, smem + static_cast<size_t>(warp) * Row::kShared);
-  uint32_t gone = 0;
   row.fetch(p, static_cast<int>(r0), r1);
   for (int r = static_cast<int>(r0); r < r1; ++r) {
     bool some = true;
     if (r < row.l.first || r >= row.l.end) {
       some = find_line(p, r, row.lane, row.l);
-      if (some) row.rules(p, &gone);
+      if (some) row.rules(p);
       else row.l.first = row.l.end = 0;
     }
     float v[Row::kLane], x[2];
@@ -485,24 +493,23 @@ __global__ void __launch_bounds__(kRulesThreads, 8) logit_rules_kernel(const __g
     row.template ruled<true>(v);
     row.pair(x);
     __syncwarp();
-    row.fetch(p, r + 1, r1);
-    if (!some) continue;
-    O* o = static_cast<O*>(p.out) + r * p.out_pitch;
-    // the dense stores cover the entries too (in place that would take the logits of those read only
-    // after them, past the 64 in registers: entries are then left out)
-    const bool spare = row.n > 64 && p.in_place;
-    const int c = row.base + row.lane * V;
+    const bool early = row.n <= 64;  // entries past the registers' are read from the row's place below
+    if (early) row.fetch(p, r + 1, r1);
+    if (some) {
+      O* o = static_cast<O*>(p.out) + r * p.out_pitch;
+      const int c = row.base + row.lane * V;
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
-      store_ruled<O, V>(o + c + j * 32 * V, v + j * V, spare ? gone >> (j * V) & ((1u << V) - 1) : 0u, p.classes - c - j * 32 * V);
-    if (row.n) {
-      __syncwarp();
-      row.entries(p, r, x, [&](float y, int k) {
-        if constexpr (sizeof(O) == 2) o[k] = __float2half_rn(y);
-        else o[k] = y;
-      });
-      __syncwarp();
+      for (int j = 0; j < NV; ++j) store_ruled<O, V>(o + c + j * 32 * V, v + j * V, p.classes - c - j * 32 * V);
+      if (row.n) {  // the entries over what the dense pass wrote
+        __syncwarp();
+        row.entries(row.place(), x, [&](float y, int k) {
+          if constexpr (sizeof(O) == 2) o[k] = __float2half_rn(y);
+          else o[k] = y;
+        });
+        __syncwarp();
+      }
     }
+    if (!early) row.fetch(p, r + 1, r1);
   }
 }
 
@@ -528,13 +535,13 @@ struct TeamRow {
 
 // A span's classes but the blank in row z (its classes from `base`), from memory: what is seldom
 // needed, by whole warps.  f(ruled logit, class); a forbidden class is -inf whatever it holds.
-template <typename T, typename F>
-__device__ __forceinline__ void span_classes(const T* z, uint8_t* shared, int span, int base, int classes, int n, float repeat,
+template <int kSpan, int kCap, typename T, typename F>
+__device__ __forceinline__ void span_classes(const T* z, uint8_t* shared, int base, int classes, int n, float repeat,
                                              const float* bias, F f) {
   const int lane = threadIdx.x % 32;
-  const SpanRules s(shared, span);
+  const SpanRules<kSpan, kCap> s(shared);
 #pragma unroll 1
-  for (int k = lane; k < span && base + k < classes; k += 32) {
+  for (int k = lane; k < kSpan && base + k < classes; k += 32) {
     const float a = s.add[k];
     if (base + k != 0 && a != -INFINITY) f(__fadd_rn(load_logit(z + k), a), base + k);
   }
@@ -544,21 +551,21 @@ __device__ __forceinline__ void span_classes(const T* z, uint8_t* shared, int sp
 }
 
 // The lane's sum of exp(z - best) where the dense pass met a NaN.
-template <typename T>
-__device__ __noinline__ float careful_sum(const T* z, uint8_t* shared, int span, int base, int classes, int n, float repeat,
+template <int kSpan, int kCap, typename T>
+__device__ __noinline__ float careful_sum(const T* z, uint8_t* shared, int base, int classes, int n, float repeat,
                                           const float* bias, float best) {
   const RowBase from(best);
   float sum = 0.0f;
-  span_classes(z, shared, span, base, classes, n, repeat, bias, [&](float y, int) { sum += from.term(y); });
+  span_classes<kSpan, kCap>(z, shared, base, classes, n, repeat, bias, [&](float y, int) { sum += from.term(y); });
   return sum;
 }
 
 // The warp's highest key below `below` (0: none).
-template <typename T>
-__device__ __noinline__ unsigned long long key_below(const T* z, uint8_t* shared, int span, int base, int classes, int n,
+template <int kSpan, int kCap, typename T>
+__device__ __noinline__ unsigned long long key_below(const T* z, uint8_t* shared, int base, int classes, int n,
                                                      float repeat, const float* bias, unsigned long long below) {
   unsigned long long k = 0;
-  span_classes(z, shared, span, base, classes, n, repeat, bias, [&](float y, int c) {
+  span_classes<kSpan, kCap>(z, shared, base, classes, n, repeat, bias, [&](float y, int c) {
     const unsigned long long u = y > -INFINITY ? class_key(y, c) : 0ull;
     if (u < below && u > k) k = u;
   });
@@ -614,13 +621,123 @@ __device__ __forceinline__ void write_candidates(const LineParams& p, int r, int
   __syncwarp();
 }
 
+// ---------------------------------------------------------------- rows that no team's registers hold
+//
+// More classes than a team's registers hold (kRegisterClasses), or a line whose history names more
+// classes of a span than its list keeps: a team takes the row in spans of kSlowSpan, each read from
+// memory as often as the row asks and its rules set anew.  Right, not fast.
+
+constexpr int kSlowSpan = 256;  // a list holds them all
+
+template <int kOp, typename T, bool kTeam>
+__device__ __noinline__ void slow_row(const LineParams& p, int r, LineRule l, TeamRow& t, uint8_t* shared, int w, int warps) {
+  const int lane = threadIdx.x % 32;
+  const T* z = static_cast<const T*>(p.z) + r * p.pitch;
+  auto sync = [&]() {
+    if constexpr (kTeam) __syncthreads();
+    else __syncwarp();
+  };
+  // f(ruled logit, class) for this warp's classes but the blank
+  auto classes = [&](auto f) {
+#pragma unroll 1
+    for (int base = w * kSlowSpan; base < p.classes; base += warps * kSlowSpan) {
+      const int n = set_rules<1, kSlowSpan / 32, kSlowSpan>(shared, p.classes, base, l.had, l.n_had, l.presence, l.frequency, l.bias,
+                                                            false, l.allowed);
+      span_classes<kSlowSpan, kSlowSpan>(z + base, shared, base, p.classes, n, l.repeat, l.bias, f);
+      __syncwarp();
+    }
+  };
+  sync();
+  if (w == 0 && lane == 0) t.listed[0] = 0;
+  float high = -INFINITY;
+  classes([&](float y, int) { high = fmaxf(high, y); });
+  const int groups = 32 / warps;
+  for (int o = 16; o >= groups; o /= 2) high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, o));
+  if (lane < groups) t.group[0][w * groups + lane] = high;
+  if (w == 0 && lane == 0) {  // the blank
+    int times = 0;
+    for (int k = 0; k < l.n_had; ++k) times += l.had[k] == 0;
+    float y = load_logit(z);
+    if (times) y = penalised(y, __fadd_rn(__fmul_rn(static_cast<float>(times), l.frequency), l.presence), l.repeat);
+    if (l.bias) y = l.bias[0] == -INFINITY ? -INFINITY : __fadd_rn(y, l.bias[0]);
+    t.blank[0] = l.allowed && !(l.allowed[0] & 1u) ? -INFINITY : y;
+  }
+  sync();
+  const float blank = t.blank[0], others = warp_max(t.group[0][lane]), best = fmaxf(others, blank);
+  const bool some = best > -INFINITY;
+  const RowBase from(best);
+  if (kOp == kOpGreedy && blank >= others) {
+    if (w == 0 && lane == 0) {
+      p.ids[r] = 0;
+      p.probs[r] = 0.0f;
+    }
+    sync();
+    return;
+  }
+  float sum = 0.0f;
+  uint32_t arg = 0xffffffffu;
+  const float reach = kOp == kOpCandidates && p.topk > 0 ? kth_group(t.group[0][lane], p.topk, lane) : INFINITY;
+  classes([&](float y, int c) {
+    sum += from.term(y);
+    if constexpr (kOp == kOpGreedy) arg = y == best ? min(arg, static_cast<uint32_t>(c)) : arg;
+    else if (y >= reach && p.topk > 0) list_key(t, 0, y, c);
+  });
+  sum = warp_sum(sum);
+  arg = __reduce_min_sync(0xffffffffu, arg);
+  if (lane == 0) {
+    t.sum[0][w] = sum;
+    t.arg[0][w] = arg;
+  }
+  sync();
+  if (kOp == kOpCandidates && t.listed[0] > kShortList) {
+    unsigned long long below = ~0ull;
+#pragma unroll 1
+    for (int q = 0; q < p.topk; ++q) {
+      unsigned long long k = 0;
+      classes([&](float y, int c) {
+        const unsigned long long u = y > -INFINITY ? class_key(y, c) : 0ull;
+        if (u < below && u > k) k = u;
+      });
+      k = warp_max_key(k);
+      if (lane == 0) t.top[w] = k;
+      sync();
+      below = warp_max_key(lane < warps ? t.top[lane] : 0ull);
+      sync();
+      if (w == 0 && lane == 0) {
+        t.list[0][q] = below;
+        t.listed[0] = q + 1;
+      }
+    }
+    sync();
+  }
+  if (w == 0) {
+    sum = warp_sum(lane < warps ? t.sum[0][lane] : 0.0f) + from.term(blank);
+    if constexpr (kOp == kOpGreedy) {
+      arg = __reduce_min_sync(0xffffffffu, lane < warps ? t.arg[0][lane] : 0xffffffffu);
+      if (lane == 0) {
+        p.ids[r] = static_cast<int32_t>(arg);
+        p.probs[r] = __fdiv_rn(from.term(best), sum);
+      }
+    } else {
+      write_candidates(p, r, lane, t, 0, blank, from, some, sum);
+    }
+  }
+  sync();
+}
+
+constexpr int kAloneWarps = 2;  // of a block whose warps take rows alone
+constexpr int kDecodeWarps = 16;  // an SM's, at 128 registers (20 at 96 spill: 79 us against 64 at 65,536 x 800)
+
 template <int kOp, typename T, int V, int NV, bool kTeam>
-__global__ void __launch_bounds__(512, 1) line_rows_kernel(const __grid_constant__ LineParams p) {
-  using Row = WarpRow<T, V, NV>;
+__global__ void __launch_bounds__(32 * kMaxTeam, 1) line_rows_kernel(const __grid_constant__ LineParams p) {
+  using Row = WarpRow<T, V, NV, kDecodeEntries>;
   extern __shared__ __align__(16) uint8_t smem[];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int w = kTeam ? warp : 0, warps = kTeam ? p.warps : 1;
-  constexpr int kTeamRow = kTeam || kOp == kOpCandidates ? sizeof(TeamRow) : 0;  // (a warp alone and greedy: unused)
+  if (kOp == kOpGreedy) launch_next();
+  constexpr bool kMayCrowd = Row::kSpan > Row::kCap;
+  constexpr int kTeamRow = kTeam || kOp == kOpCandidates || kMayCrowd ? sizeof(TeamRow) : 0;
+  static_assert(!kMayCrowd || Row::kRules >= SpanRules<kSlowSpan, kSlowSpan>::kBytes, "");
   const long long team = kTeam ? blockIdx.x : static_cast<long long>(blockIdx.x) * (blockDim.x / 32) + warp;
   TeamRow& t = *reinterpret_cast<TeamRow*>(smem + (kTeam ? 0 : warp * (kTeamRow + Row::kShared)));
   const long long r0 = team * p.team_rows;
@@ -635,13 +752,27 @@ __global__ void __launch_bounds__(512, 1) line_rows_kernel(const __grid_constant
   row.start(p, w * Row::kSpan, reinterpret_cast<uint8_t*>(&t) + kTeamRow + w * Row::kShared);
   row.fetch(p, static_cast<int>(r0), r1);
   int parity = 0;
+  bool crowded = false;  // the line's entries do not fit some warp's list
 #pragma unroll 1
   for (int r = static_cast<int>(r0); r < r1; ++r) {
     bool found = true;
     if (r < row.l.first || r >= row.l.end) {
       found = find_line(p, r, lane, row.l);  // the same for every warp of the team
-      if (found) row.rules(p, nullptr);
+      if (found) row.rules(p);
       else row.l.first = row.l.end = 0;
+      if constexpr (kMayCrowd) {
+        crowded = found && row.n > Row::kCap;
+        if constexpr (kTeam) crowded = __syncthreads_or(crowded);
+        if (crowded) row.n = 0;
+      }
+    }
+    if constexpr (kMayCrowd) {
+      if (crowded) {
+        row.arrived();
+        row.fetch(p, r + 1, r1);
+        slow_row<kOp, T, kTeam>(p, r, row.l, t, row.shared, w, warps);
+        continue;
+      }
     }
     float v[Row::kLane], x[2];
     row.arrived();
@@ -672,7 +803,7 @@ __global__ void __launch_bounds__(512, 1) line_rows_kernel(const __grid_constant
         for (int j = 0; j + s < NV; j += 2 * s) m[j] = fmaxf(m[j], m[j + s]);
       high = fmaxf(m[0], -INFINITY);
     }
-    row.entries(p, r, x, [&](float y, int c) {
+    row.entries(row.row(p, r), x, [&](float y, int c) {
       if (c == 0) blank = y;
       else high = fmaxf(high, y);
     });
@@ -712,12 +843,12 @@ __global__ void __launch_bounds__(512, 1) line_rows_kernel(const __grid_constant
       const float2 d = fma2(make_float2(v[i], v[i + 1]), make_float2(kLog2e, kLog2e), make_float2(-from.c, -from.c));
       s[i / 2 % 2] = fadd2_rn(s[i / 2 % 2], make_float2(ex2_approx(d.x), ex2_approx(d.y)));
     }
-    row.entries(p, r, x, [&](float y, int c) {
+    row.entries(row.row(p, r), x, [&](float y, int c) {
       if (c != 0) s[0].x += exp_less(y, from.c);
     });
     float sum = warp_sum((s[0].x + s[0].y) + (s[1].x + s[1].y));
     if (sum != sum || !from.fits)  // a NaN or +inf met a -inf (or one is allowed), or c overflowed
-      sum = warp_sum(careful_sum(row.row(p, r), row.shared, Row::kSpan, row.base, p.classes, row.n, row.l.repeat, row.l.bias, best));
+      sum = warp_sum(careful_sum<Row::kSpan, Row::kCap>(row.row(p, r), row.shared, row.base, p.classes, row.n, row.l.repeat, row.l.bias, best));
     uint32_t arg = 0xffffffffu;
     if constexpr (kOp == kOpGreedy) {
       if (high == best) {
@@ -727,7 +858,7 @@ __global__ void __launch_bounds__(512, 1) line_rows_kernel(const __grid_constant
 #pragma unroll
           for (int i = V - 1; i >= 0; --i) c = v[j * V + i] == best ? j * 32 * V + i : c;
         if (c != 0xffffffffu) arg = row.base + lane * V + c;
-        row.entries(p, r, x, [&](float y, int k) {
+        row.entries(row.row(p, r), x, [&](float y, int k) {
           if (y == best && k != 0) arg = min(arg, static_cast<uint32_t>(k));
         });
       }
@@ -761,7 +892,7 @@ __global__ void __launch_bounds__(512, 1) line_rows_kernel(const __grid_constant
             m &= m - 1;
             list_key(t, parity, __fadd_rn(load_logit(row.row(p, r) + k), reinterpret_cast<const float*>(row.shared)[k]), row.base + k);
           }
-          row.entries(p, r, x, [&](float y, int k) {
+          row.entries(row.row(p, r), x, [&](float y, int k) {
             if (y >= reach && k != 0) list_key(t, parity, y, k);
           });
         }
@@ -773,7 +904,7 @@ __global__ void __launch_bounds__(512, 1) line_rows_kernel(const __grid_constant
 #pragma unroll 1
         for (int q = 0; q < p.topk; ++q) {
           unsigned long long k =
-              key_below(row.row(p, r), row.shared, Row::kSpan, row.base, p.classes, row.n, row.l.repeat, row.l.bias, below);
+              key_below<Row::kSpan, Row::kCap>(row.row(p, r), row.shared, row.base, p.classes, row.n, row.l.repeat, row.l.bias, below);
           if constexpr (kTeam) {
             if (lane == 0) t.top[w] = k;
             team_sync();
@@ -797,147 +928,78 @@ __global__ void __launch_bounds__(512, 1) line_rows_kernel(const __grid_constant
   }
 }
 
-// ---------------------------------------------------------------- rows that no team's registers hold
-//
-// More than kRegisterClasses classes: a block a row, its classes in passes of the same spans, each read
-// from memory as often as the row asks (and its rules set anew): right, not fast.
-
 constexpr int kRegisterClasses = kMaxTeam * 32 * kDecodeLane;
-constexpr int kWideSpan = 32 * kDecodeLane;
 
 template <int kOp, typename T>
 __global__ void __launch_bounds__(32 * kMaxTeam) wide_rows_kernel(const __grid_constant__ LineParams p) {
   extern __shared__ __align__(16) uint8_t smem[];
-  TeamRow& t = *reinterpret_cast<TeamRow*>(smem);
-  const int w = threadIdx.x / 32, lane = threadIdx.x % 32, r = blockIdx.x;
-  uint8_t* shared = smem + sizeof(TeamRow) + static_cast<size_t>(w) * kWideSpan * 10;
+  const int w = threadIdx.x / 32;
   LineRule l;
-  if (!find_line(p, r, lane, l)) return;
-  if (threadIdx.x == 0) t.listed[0] = 0;
-  const T* z = static_cast<const T*>(p.z) + r * p.pitch;
-  // f(ruled logit, class) for this warp's classes but the blank
-  auto classes = [&](auto f) {
-#pragma unroll 1
-    for (int base = w * kWideSpan; base < p.classes; base += kMaxTeam * kWideSpan) {
-      const int n = set_rules<1, kDecodeLane>(shared, p.classes, base, l.had, l.n_had, l.presence, l.frequency, l.bias, false,
-                                              l.allowed, nullptr);
-      span_classes(z + base, shared, kWideSpan, base, p.classes, n, l.repeat, l.bias, f);
-      __syncwarp();
-    }
-  };
-  float high = -INFINITY;
-  classes([&](float y, int) { high = fmaxf(high, y); });
-  for (int o = 16; o >= 2; o /= 2) high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, o));
-  if (lane < 2) t.group[0][w * 2 + lane] = high;
-  if (threadIdx.x == 0) {  // the blank
-    int times = 0;
-    for (int k = 0; k < l.n_had; ++k) times += l.had[k] == 0;
-    float y = load_logit(z);
-    if (times) y = penalised(y, __fadd_rn(__fmul_rn(static_cast<float>(times), l.frequency), l.presence), l.repeat);
-    if (l.bias) y = l.bias[0] == -INFINITY ? -INFINITY : __fadd_rn(y, l.bias[0]);
-    t.blank[0] = l.allowed && !(l.allowed[0] & 1u) ? -INFINITY : y;
-  }
-  __syncthreads();
-  const float blank = t.blank[0], others = warp_max(t.group[0][lane]), best = fmaxf(others, blank);
-  const bool some = best > -INFINITY;
-  const RowBase from(best);
-  if (kOp == kOpGreedy && blank >= others) {
-    if (threadIdx.x == 0) {
-      p.ids[r] = 0;
-      p.probs[r] = 0.0f;
-    }
-    return;
-  }
-  float sum = 0.0f;
-  uint32_t arg = 0xffffffffu;
-  const float reach = kOp == kOpCandidates && p.topk > 0 ? kth_group(t.group[0][lane], p.topk, lane) : INFINITY;
-  classes([&](float y, int c) {
-    sum += from.term(y);
-    if constexpr (kOp == kOpGreedy) arg = y == best ? min(arg, static_cast<uint32_t>(c)) : arg;
-    else if (y >= reach && p.topk > 0) list_key(t, 0, y, c);
-  });
-  sum = warp_sum(sum);
-  arg = __reduce_min_sync(0xffffffffu, arg);
-  if (lane == 0) {
-    t.sum[0][w] = sum;
-    t.arg[0][w] = arg;
-  }
-  __syncthreads();
-  if (kOp == kOpCandidates && t.listed[0] > kShortList) {
-    unsigned long long below = ~0ull;
-#pragma unroll 1
-    for (int q = 0; q < p.topk; ++q) {
-      unsigned long long k = 0;
-      classes([&](float y, int c) {
-        const unsigned long long u = y > -INFINITY ? class_key(y, c) : 0ull;
-        if (u < below && u > k) k = u;
-      });
-      k = warp_max_key(k);
-      if (lane == 0) t.top[w] = k;
-      __syncthreads();
-      below = warp_max_key(lane < kMaxTeam ? t.top[lane] : 0ull);
-      __syncthreads();
-      if (threadIdx.x == 0) {
-        t.list[0][q] = below;
-        t.listed[0] = q + 1;
-      }
-    }
-    __syncthreads();
-  }
-  if (w != 0) return;
-  sum = warp_sum(lane < kMaxTeam ? t.sum[0][lane] : 0.0f) + from.term(blank);
-  if constexpr (kOp == kOpGreedy) {
-    arg = __reduce_min_sync(0xffffffffu, lane < kMaxTeam ? t.arg[0][lane] : 0xffffffffu);
-    if (lane == 0) {
-      p.ids[r] = static_cast<int32_t>(arg);
-      p.probs[r] = __fdiv_rn(from.term(best), sum);
-    }
-  } else {
-    write_candidates(p, r, lane, t, 0, blank, from, some, sum);
-  }
+  if (kOp == kOpGreedy) launch_next();
+  if (!find_line(p, blockIdx.x, threadIdx.x % 32, l)) return;
+  slow_row<kOp, T, true>(p, blockIdx.x, l, *reinterpret_cast<TeamRow*>(smem),
+                         smem + sizeof(TeamRow) + w * SpanRules<kSlowSpan, kSlowSpan>::kBytes, w, kMaxTeam);
 }
 
 // Greedy CTC's second half, a warp a line, in place: ids and probs hold each frame's class and
 // probability; the characters go to the front of the line's places (never past the frames already
-// read), the rest is filled.
+// read), the rest is filled.  The frames of four steps are read at once: their latency, not their
+// bytes, is what this kernel takes.
 __global__ void __launch_bounds__(128) collapse_lines_kernel(const __grid_constant__ LineParams p) {
   const int i = blockIdx.x * 4 + threadIdx.x / 32, lane = threadIdx.x % 32;
+  int first = 0, end = 0;
+  if (i < p.lines) {
+    first = min(max(p.line_at[i], 0), p.rows);
+    end = min(max(p.line_at[i + 1], first), p.rows);
+  }
+  launch_wait();  // the frames' kernel is done
   if (i >= p.lines) return;
-  const int first = min(max(p.line_at[i], 0), p.rows), end = min(max(p.line_at[i + 1], first), p.rows);
-  int prev = 0;       // the class of the frame before
-  int k = 0;          // characters so far
+  constexpr int kSteps = 4;
+  const uint32_t upto = 0xffffffffu >> (31 - lane);
+  int prev = 0;        // the class of the frame before
+  int k = 0;           // characters so far
   float carry = 0.0f;  // the last character's highest probability, where it may go on
-  for (int t0 = first; t0 < end; t0 += 32) {
-    const int t = t0 + lane;
-    const int id = t < end ? p.ids[t] : 0;
-    float pr = t < end ? p.probs[t] : 0.0f;
-    int before = __shfl_up_sync(0xffffffffu, id, 1);
-    if (lane == 0) before = prev;
-    const bool goes_on = id != 0 && id == before;
-    const unsigned begins = __ballot_sync(0xffffffffu, id != 0 && id != before);
-    // the highest probability up to this frame of the frames of its character
-    for (int o = 1; o < 32; o <<= 1) {
-      const float up = __shfl_up_sync(0xffffffffu, pr, o);
-      const unsigned between = lane >= o ? begins & (0xffffffffu >> (31 - lane)) & ~(0xffffffffu >> (31 - (lane - o))) : 1u;
-      const int uid = __shfl_up_sync(0xffffffffu, id, o);
-      if (lane >= o && between == 0 && uid == id) pr = up > pr ? up : pr;
+  for (int t0 = first; t0 < end; t0 += 32 * kSteps) {
+    int ids[kSteps];
+    float prs[kSteps];
+#pragma unroll
+    for (int u = 0; u < kSteps; ++u) {
+      const int t = t0 + 32 * u + lane;
+      ids[u] = t < end ? p.ids[t] : 0;
+      prs[u] = t < end ? p.probs[t] : 0.0f;
     }
-    const unsigned mine = begins & (0xffffffffu >> (31 - lane));
-    const bool from_before = goes_on && mine == 0;
-    if (from_before) pr = carry > pr ? carry : pr;
-    const int after = __shfl_down_sync(0xffffffffu, id, 1);
-    const bool last = id != 0 && (lane == 31 || after != id);
-    const int nth = k + __popc(mine) - 1;
     __syncwarp();
-    if (last) {
-      p.ids[first + nth] = id;
-      p.probs[first + nth] = pr;
+#pragma unroll
+    for (int u = 0; u < kSteps; ++u) {
+      if (t0 + 32 * u >= end) break;
+      const int id = ids[u];
+      float pr = prs[u];
+      int before = __shfl_up_sync(0xffffffffu, id, 1);
+      if (lane == 0) before = prev;
+      const unsigned begins = __ballot_sync(0xffffffffu, id != 0 && id != before);
+      const unsigned mine = begins & upto;
+      if (__any_sync(0xffffffffu, id != 0 && id == before)) {
+        // the highest probability up to this frame of the frames of its character
+        for (int o = 1; o < 32; o <<= 1) {
+          const float up = __shfl_up_sync(0xffffffffu, pr, o);
+          const int uid = __shfl_up_sync(0xffffffffu, id, o);
+          if (lane >= o && uid == id && (mine & ~(upto >> o)) == 0) pr = up > pr ? up : pr;
+        }
+        if (id != 0 && id == before && mine == 0) pr = carry > pr ? carry : pr;
+      }
+      const int after = __shfl_down_sync(0xffffffffu, id, 1);
+      const bool last = id != 0 && (lane == 31 || after != id);
+      const int nth = k + __popc(mine) - 1;
+      if (last) {
+        p.ids[first + nth] = id;
+        p.probs[first + nth] = pr;
+      }
+      if (begins >> lane & 1) p.starts[first + nth] = t0 + 32 * u + lane - first;
+      k += __popc(begins);
+      prev = __shfl_sync(0xffffffffu, id, 31);
+      carry = __shfl_sync(0xffffffffu, pr, 31);
+      __syncwarp();
     }
-    if (begins >> lane & 1) p.starts[first + nth] = t - first;
-    k += __popc(begins);
-    prev = __shfl_sync(0xffffffffu, id, 31);
-    carry = __shfl_sync(0xffffffffu, pr, 31);
-    __syncwarp();
   }
   for (int t = first + k + lane; t < end; t += 32) {
     p.ids[t] = -1;

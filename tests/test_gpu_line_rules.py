@@ -329,6 +329,42 @@ def test_history_of_a_long_line():
     c.check_greedy()
 
 
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("classes", [300, 800, 2000, 12000])
+def test_a_history_that_names_every_class(classes, half):
+    """More distinct characters than any list of them keeps, in some lines and not in others."""
+    rng = np.random.default_rng(classes)
+    lengths = [9, 2, 1, 12]
+    at = line_places(rng, lengths)
+    ids = [rng.permutation(classes), rng.integers(0, classes, 50), np.concatenate([np.arange(classes), np.arange(0, classes, 3)]),
+           rng.integers(0, classes, 5)]
+    rules = some_rules(rng, 4, classes)
+    rules["history"] = np.concatenate(ids).astype(np.int32)
+    rules["history_at"] = np.concatenate([[0], np.cumsum([len(i) for i in ids])]).astype(np.int32)
+    c = Case(logits_of(rng, at[-1], classes, half), at, rules)
+    c.check_ruled()
+    c.check_greedy()
+    c.check_candidates(16)
+    native.logit_rules(c.frames, c.crules, c.frames.logits, c.kind)  # in place
+    c.torch.cuda.synchronize()
+    with np.errstate(over="ignore"):
+        assert np.array_equal(c.keep[0].cpu().numpy().reshape(-1, classes), c.want.astype(c.z.dtype), equal_nan=True)
+
+
+def test_the_types_lowest_value_everywhere():
+    """Rows of the lowest value, as callers mask: a maximum that times log2 e overflows."""
+    z = np.full((4, 900), np.finfo(np.float32).min, np.float32)
+    z[1, 5] = np.finfo(np.float32).max / 2
+    z[2, 700:] = -1
+    z[3, 1:] *= np.float32(0.5)
+    c = Case(z, np.array([0, 4], np.int32), None)
+    c.check_greedy()
+    c.check_candidates(3)
+    c = Case(np.tile(z, (1, 3)), np.array([0, 4], np.int32), None)
+    c.check_greedy()
+    c.check_candidates(3)
+
+
 def test_in_place_and_side_by_side():
     import torch
     rng = np.random.default_rng(3)
