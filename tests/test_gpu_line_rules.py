@@ -151,6 +151,8 @@ class Case:
         tol = R.sum_tolerance(self.z.shape[1])
 
         def near(a, b):
+            with np.errstate(over="ignore"):  # what float32 cannot hold is an infinity
+                b = np.where(np.isinf(b.astype(np.float32)), b.astype(np.float32), b)
             fin = np.isfinite(b)
             # the sizes in play: z - best at most |logp| + ln C, ln sum at most ln C, the result itself
             room = tol + 2.0 ** -24 * (2 * np.abs(b[fin]) + 4 * np.log(self.z.shape[1] + 1) + 1)
