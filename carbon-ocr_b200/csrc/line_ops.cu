@@ -188,6 +188,22 @@ cudaError_t decode(LineParams& p, cudaStream_t s) {
   else return decode_fit<kOp, T, V>(p, need, sms, s, std::integer_sequence<int, 4, 16, 32>{});
 }
 
+// Long rows where lines are long too: a block sets a line's rules for 16 warps, so from 16 frames a line
+// on average (fewer leave warps idle and pay the rules more often than a team of 16 does).
+constexpr int kLongLines = 16;
+
+template <int kOp, typename T, int V>
+cudaError_t decode_long(LineParams& p, cudaStream_t s) {
+  using L = LongRow<T, V>;
+  int sms = 0;
+  const cudaError_t e = sm_count(&sms);
+  if (e != cudaSuccess) return e;
+  const int chunks = (p.classes + L::kChunk - 1) / L::kChunk;
+  p.team_rows = (p.rows + sms - 1) / sms;
+  const size_t smem = sizeof(TeamRow) + kLongEntries * 10 + static_cast<size_t>(chunks) * L::kChunk * 4 + kMaxTeam * L::kWarp;
+  return launch_on(long_rows_kernel<kOp, T, V>, p, (p.rows + p.team_rows - 1) / p.team_rows, 32 * kMaxTeam, smem, s);
+}
+
 template <int kOp, typename T>
 cudaError_t decode_wide(LineParams& p, cudaStream_t s) {
   return launch_on(wide_rows_kernel<kOp, T>, p, p.rows, 32 * kMaxTeam,
@@ -225,6 +241,10 @@ template <int kOp>
 cudaError_t launch_decode(LineParams& p, int type, cudaStream_t s) {
   bias_reads(p);
   if (p.classes > kRegisterClasses) return type == CREC_FP16 ? decode_wide<kOp, __half>(p, s) : decode_wide<kOp, float>(p, s);
+  if (p.classes > 32 * kDecodeLane && p.rows / p.lines >= kLongLines) {
+    if (type == CREC_FP16) return wide(p.z, p.pitch, 2, 16) ? decode_long<kOp, __half, 8>(p, s) : decode_long<kOp, __half, 1>(p, s);
+    return wide(p.z, p.pitch, 4, 16) ? decode_long<kOp, float, 4>(p, s) : decode_long<kOp, float, 1>(p, s);
+  }
   if (type == CREC_FP16)
     return wide(p.z, p.pitch, 2, 16) ? decode<kOp, __half, 8>(p, s) : decode<kOp, __half, 1>(p, s);
   return wide(p.z, p.pitch, 4, 16) ? decode<kOp, float, 4>(p, s) : decode<kOp, float, 1>(p, s);

@@ -289,10 +289,16 @@ __device__ __noinline__ int set_rules(uint8_t* shared, int classes, int base, co
       if (c >= 0 && c < kSpan) atomicAdd(&count[c], 1u);
     }
     __syncwarp();
-    // each class once: whoever takes its count makes the entry
+    // each class once, by the first lane that has it of the first step that does: the entries' order,
+    // and with it the order of every sum over them, is the history's
     for (int k0 = 0; k0 < n_had; k0 += 32) {
       const int c = k0 + lane < n_had ? had[k0 + lane] - base : -1;
-      const uint32_t times = c >= 0 && c < kSpan ? atomicExch(&count[c], 0u) : 0u;
+      const unsigned same = __match_any_sync(0xffffffffu, c);
+      const bool takes = c >= 0 && c < kSpan && (same & ((1u << lane) - 1)) == 0;
+      const uint32_t times = takes ? count[c] : 0u;
+      __syncwarp();
+      if (takes) count[c] = 0;
+      __syncwarp();
       const bool left_out = times && (base + c >= classes || (allowed && !(allowed[(base + c) >> 5] >> ((base + c) & 31) & 1)) ||
                                       (bias && bias[base + c] == -INFINITY));
       const unsigned m = __ballot_sync(0xffffffffu, times && !left_out);
@@ -925,6 +931,370 @@ __global__ void __launch_bounds__(32 * kMaxTeam, 1) line_rows_kernel(const __gri
       }
     }
     parity ^= 1;
+  }
+}
+
+// ---------------------------------------------------------------- long rows
+//
+// More than 1,024 classes, many frames a line: a warp a row all the same, a block of 16 warps a line's
+// rows.  The line's rules on all classes lie in shared memory once for the block; a row comes through
+// its warp in chunks, three places deep, with the maximum and the sum of exp(z - base) kept as it goes
+// (the base, one for the warp, rises with the maximum, and the sum is scaled by the bases' exact
+// difference).  No barrier a row: teams of 16 warps that meet twice a row took 3 times as long
+// (4,096 x 12,000 float16: 127 us).  Candidates are listed as they reach what the lanes' maxima so far
+// promise of the k-th highest, and the list is cut to what the last promise leaves before it is ranked.
+
+constexpr int kLongEntries = 256;  // of a line; one with more goes the slow way
+constexpr int kLongList = 128;     // keys of a row
+constexpr int kLongPlaces = 3;
+
+template <typename T, int V>
+struct LongRow {
+  static constexpr int NV = V == 1 ? 16 : 4, kLane = NV * V, kChunk = 32 * kLane;
+  static constexpr int kWarp = kLongPlaces * kChunk * static_cast<int>(sizeof(T)) + kLongList * 8;  // shared bytes of a warp
+};
+
+template <int kOp, typename T, int V>
+__global__ void __launch_bounds__(32 * kMaxTeam, 1) long_rows_kernel(const __grid_constant__ LineParams p) {
+  using L = LongRow<T, V>;
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ int s_n;
+  const int w = threadIdx.x / 32, lane = threadIdx.x % 32;
+  if (kOp == kOpGreedy) launch_next();
+  const int chunks = (p.classes + L::kChunk - 1) / L::kChunk;
+  TeamRow& t = *reinterpret_cast<TeamRow*>(smem);
+  float* less = reinterpret_cast<float*>(smem + sizeof(TeamRow));  // the entries
+  float* plus = less + kLongEntries;
+  uint16_t* at = reinterpret_cast<uint16_t*>(plus + kLongEntries);
+  float* add = reinterpret_cast<float*>(at + kLongEntries);  // [chunks * kChunk]
+  uint8_t* mine = reinterpret_cast<uint8_t*>(add + chunks * L::kChunk) + w * L::kWarp;
+  T* places = reinterpret_cast<T*>(mine);
+  unsigned long long* list = reinterpret_cast<unsigned long long*>(mine + kLongPlaces * L::kChunk * sizeof(T));
+  auto clear = [&]() {  // past the last class: 0 (its add is -inf)
+    for (int k = lane; k < kLongPlaces * L::kChunk; k += 32) places[k] = T(0.0f);
+    __syncwarp();
+  };
+  clear();
+  const int b0 = static_cast<int>(min(static_cast<long long>(p.rows), static_cast<long long>(blockIdx.x) * p.team_rows));
+  const int b1 = static_cast<int>(min(static_cast<long long>(p.rows), static_cast<long long>(b0) + p.team_rows));
+  int r = b0;
+  while (r < b1) {
+    LineRule l;
+    if (!find_line(p, r, lane, l)) {  // the same for every warp
+      ++r;
+      continue;
+    }
+    const int end = min(l.end, b1);
+    // the fetches run ahead of the rows: (f_row, f_chunk) next
+    int f_row = r + w, f_chunk = 0, f_place = 0;
+    auto fetch = [&]() {
+      if (f_row < end) {
+        const int c = f_chunk * L::kChunk + lane * V;
+        const T* z = static_cast<const T*>(p.z) + f_row * p.pitch + c;
+        T* s = places + f_place * L::kChunk + lane * V;
+        const int left = p.classes - c;
+#pragma unroll
+        for (int j = 0; j < L::NV; ++j) {
+          if constexpr (V * sizeof(T) >= 4) {
+            if (j * 32 * V < left)
+              copy_async<V * sizeof(T)>(s + j * 32 * V, z + j * 32 * V, min(V, left - j * 32 * V) * static_cast<int>(sizeof(T)));
+          } else {
+            if (j * 32 * V < left) s[j * 32 * V] = z[j * 32 * V];
+          }
+        }
+        if (++f_chunk == chunks) {
+          f_chunk = 0;
+          f_row += kMaxTeam;
+        }
+      }
+      f_place = f_place + 1 == kLongPlaces ? 0 : f_place + 1;
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    for (int k = 0; k < kLongPlaces; ++k) fetch();
+    // the line's rules
+    __syncthreads();  // the rows before are done with the last line's
+    uint32_t* count = reinterpret_cast<uint32_t*>(add);
+    int n = 0;
+    if (l.n_had > 0) {
+      for (int c = threadIdx.x; c < p.classes; c += blockDim.x) count[c] = 0;
+      __syncthreads();
+      for (int k = threadIdx.x; k < l.n_had; k += blockDim.x) {
+        const int c = l.had[k];
+        if (c >= 0 && c < p.classes) atomicAdd(&count[c], 1u);
+      }
+      __syncthreads();
+      if (w == 0) {
+        for (int k0 = 0; k0 < l.n_had; k0 += 32) {
+          const int c = k0 + lane < l.n_had ? l.had[k0 + lane] : -1;
+          const unsigned same = __match_any_sync(0xffffffffu, c);
+          const bool takes = c >= 0 && c < p.classes && (same & ((1u << lane) - 1)) == 0;
+          const uint32_t times = takes ? count[c] : 0u;
+          __syncwarp();
+          if (takes) count[c] = 0;
+          __syncwarp();
+          const float b = times && l.bias ? l.bias[c] : 0.0f;
+          const bool keeps = times && b != -INFINITY && (!l.allowed || (l.allowed[c >> 5] >> (c & 31) & 1));
+          const unsigned m = __ballot_sync(0xffffffffu, keeps);
+          const int e = n + __popc(m & ((1u << lane) - 1));
+          if (keeps && e < kLongEntries) {
+            at[e] = static_cast<uint16_t>(c);
+            less[e] = __fadd_rn(__fmul_rn(static_cast<float>(times), l.frequency), l.presence);
+            plus[e] = b;
+          }
+          n += __popc(m);
+        }
+        if (lane == 0) s_n = n;
+      }
+      __syncthreads();
+      n = s_n;
+    }
+    for (int c = threadIdx.x; c < chunks * L::kChunk; c += blockDim.x)
+      add[c] = c < p.classes && (!l.allowed || (l.allowed[c >> 5] >> (c & 31) & 1)) ? (l.bias ? l.bias[c] : 0.0f) : -INFINITY;
+    __syncthreads();
+    if (n <= kLongEntries) {
+      for (int e = threadIdx.x; e < n; e += blockDim.x) add[at[e]] = -INFINITY;
+    }
+    __syncthreads();
+    if (n > kLongEntries) {
+      copy_wait_all();
+      __syncthreads();
+      for (; r < end; ++r) slow_row<kOp, T, true>(p, r, l, t, reinterpret_cast<uint8_t*>(add) + w * SpanRules<kSlowSpan, kSlowSpan>::kBytes, w, kMaxTeam);
+      clear();  // (slow rows work in the table and in what follows it)
+      continue;
+    }
+
+    int place = 0;
+#pragma unroll 1
+    for (int row = r + w; row < end; row += kMaxTeam) {
+      const T* z = static_cast<const T*>(p.z) + row * p.pitch;
+      // the entries first (at most 8 a lane); the blank apart
+      float blank = -INFINITY, high = -INFINITY, x[kLongEntries / 32];
+#pragma unroll
+      for (int i = 0; i < kLongEntries / 32; ++i) {
+        x[i] = -INFINITY;
+        if (32 * i >= n) continue;
+        const int e = 32 * i + lane;
+        if (e >= n) continue;
+        x[i] = __fadd_rn(penalised(load_logit(z + at[e]), less[e], l.repeat), plus[e]);
+        if (at[e] == 0) {
+          blank = x[i];
+          x[i] = -INFINITY;
+        }
+        high = fmaxf(high, x[i]);
+      }
+      float best = warp_max(high), reach = INFINITY;
+      uint32_t arg = 0xffffffffu;
+      int listed = 0;
+      float2 s[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+      float c = __fmul_rn(best == -INFINITY ? 0.0f : best, kLog2e);
+      bool based = best > -INFINITY;  // c belongs to a logit
+      auto push = [&](bool takes, float y, int k) {  // by whole warps
+        const unsigned m = __ballot_sync(0xffffffffu, takes);
+        const int to = listed + __popc(m & ((1u << lane) - 1));
+        if (takes && to < kLongList) list[to] = class_key(y, k);
+        listed += __popc(m);
+      };
+#pragma unroll
+      for (int i = 0; i < kLongEntries / 32; ++i) {
+        if (32 * i >= n) continue;
+        s[0].x += exp_less(x[i], c);
+        if constexpr (kOp == kOpGreedy) {
+          if (x[i] == best && best > -INFINITY) arg = min(arg, static_cast<uint32_t>(at[32 * i + lane]));
+        }
+      }
+      if constexpr (kOp == kOpGreedy) arg = __reduce_min_sync(0xffffffffu, arg);
+#pragma unroll 1
+      for (int chunk = 0; chunk < chunks; ++chunk) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kLongPlaces - 1) : "memory");
+        __syncwarp();
+        float v[L::kLane];
+        const float* a = add + chunk * L::kChunk + lane * V;
+        const T* q = places + place * L::kChunk + lane * V;
+#pragma unroll
+        for (int j = 0; j < L::NV; ++j) {
+          float u[V];
+          get_logits<V>(q + j * 32 * V, u);
+          if constexpr (V == 1) {
+            v[j] = __fadd_rn(u[0], a[j * 32]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < V; i += 4) {
+              const float4 f = *reinterpret_cast<const float4*>(a + j * 32 * V + i);
+              const float2 d0 = fadd2_rn(make_float2(u[i], u[i + 1]), make_float2(f.x, f.y));
+              const float2 d1 = fadd2_rn(make_float2(u[i + 2], u[i + 3]), make_float2(f.z, f.w));
+              v[j * V + i] = d0.x;
+              v[j * V + i + 1] = d0.y;
+              v[j * V + i + 2] = d1.x;
+              v[j * V + i + 3] = d1.y;
+            }
+          }
+        }
+        if (chunk == 0 && lane == 0) {
+          if (add[0] != -INFINITY) blank = v[0];
+          v[0] = -INFINITY;
+        }
+        float m = v[0];
+#pragma unroll
+        for (int i = 1; i < L::kLane; ++i) m = fmaxf(m, v[i]);
+        high = fmaxf(high, m);
+        const float top = warp_max(m);
+        if (top > best) {
+          if constexpr (kOp == kOpGreedy) {
+            uint32_t k = 0xffffffffu;
+            if (m == top) {
+#pragma unroll
+              for (int j = L::NV - 1; j >= 0; --j)
+#pragma unroll
+                for (int i = V - 1; i >= 0; --i) k = v[j * V + i] == top ? chunk * L::kChunk + (j * 32 + lane) * V + i : k;
+            }
+            arg = __reduce_min_sync(0xffffffffu, k);
+          }
+          best = top;
+          const float c2 = __fmul_rn(best, kLog2e);
+          const float f = based ? ex2_approx(__fsub_rn(c, c2)) : 0.0f;
+          s[0].x = based ? s[0].x * f : s[0].x;
+          s[0].y = based ? s[0].y * f : s[0].y;
+          s[1].x = based ? s[1].x * f : s[1].x;
+          s[1].y = based ? s[1].y * f : s[1].y;
+          c = c2;
+          based = true;
+        } else if (kOp == kOpGreedy && top == best && top > -INFINITY) {
+          // an entry's class may lie behind an equal one of the dense pass
+          uint32_t k = 0xffffffffu;
+#pragma unroll
+          for (int j = L::NV - 1; j >= 0; --j)
+#pragma unroll
+            for (int i = V - 1; i >= 0; --i) k = v[j * V + i] == top ? chunk * L::kChunk + (j * 32 + lane) * V + i : k;
+          arg = min(arg, __reduce_min_sync(0xffffffffu, k));
+        }
+#pragma unroll
+        for (int i = 0; i < L::kLane; i += 2) {
+          const float2 d = fma2(make_float2(v[i], v[i + 1]), make_float2(kLog2e, kLog2e), make_float2(-c, -c));
+          s[i / 2 % 2] = fadd2_rn(s[i / 2 % 2], make_float2(ex2_approx(d.x), ex2_approx(d.y)));
+        }
+        if (kOp == kOpCandidates && p.topk > 0) {
+          if ((chunk & (chunk + 1)) == 0) reach = kth_group(high, p.topk, lane);  // chunks 0, 1, 3, 7, ...
+          if (__any_sync(0xffffffffu, m >= reach)) {
+            uint32_t bits = 0;
+            if (m >= reach) {
+#pragma unroll
+              for (int i = 0; i < L::kLane; ++i) bits |= static_cast<uint32_t>(v[i] >= reach) << i;
+            }
+            while (__any_sync(0xffffffffu, bits != 0)) {  // a lane's lowest at a time, read again from its place
+              const int i = max(__ffs(bits) - 1, 0), k = (i / V * 32 + lane) * V + i % V;
+              push(bits != 0, __fadd_rn(load_logit(places + place * L::kChunk + k), add[chunk * L::kChunk + k]), chunk * L::kChunk + k);
+              bits &= bits - 1;
+            }
+          }
+        }
+        __syncwarp();
+        place = place + 1 == kLongPlaces ? 0 : place + 1;
+        fetch();
+      }
+      blank = warp_max_nan(blank);
+      if (kOp == kOpGreedy && blank >= best) {
+        if (lane == 0) {
+          p.ids[row] = 0;
+          p.probs[row] = 0.0f;
+        }
+        continue;
+      }
+      const float all = fmaxf(best, blank);
+      const bool some = all > -INFINITY;
+      const RowBase from(all);
+      float sum = warp_sum((s[0].x + s[0].y) + (s[1].x + s[1].y));
+      if (sum != sum || !from.fits || !(fabsf(c) < 1048576.0f)) {
+        // a NaN or +inf met a -inf (or is allowed), or a base was too large: from memory, by differences
+        sum = 0.0f;
+#pragma unroll 1
+        for (int k = lane; k < p.classes; k += 32)
+          if (k != 0 && add[k] != -INFINITY) sum += from.term(__fadd_rn(load_logit(z + k), add[k]));
+#pragma unroll
+        for (int i = 0; i < kLongEntries / 32; ++i) sum += from.term(x[i]);
+        sum = warp_sum(sum);
+      } else if (best > -INFINITY) {
+        sum *= ex2_approx(__fsub_rn(c, from.c));  // from the highest of the others to the row's base
+      }
+      sum += from.term(blank);
+      if constexpr (kOp == kOpGreedy) {
+        if (lane == 0) {
+          p.ids[row] = static_cast<int32_t>(arg);
+          p.probs[row] = __fdiv_rn(from.term(all), sum);
+        }
+      } else {
+        const float ln = some ? logf(__fdiv_rn(sum, from.term(from.best))) : sum;
+        const size_t o = static_cast<size_t>(row) * p.topk;
+        if (p.topk > 0) {
+          __syncwarp();
+          unsigned long long key[kLongList / 32];  // what the last promise leaves, moved to the front
+          reach = kth_group(high, p.topk, lane);
+#pragma unroll
+          for (int i = 0; i < kLongEntries / 32; ++i)
+            if (32 * i < n) push(x[i] >= reach, x[i], 32 * i + lane < n ? at[32 * i + lane] : 0);
+          __syncwarp();
+          if (listed <= kLongList) {
+            const unsigned long long least = static_cast<unsigned long long>(float_order(reach)) << 32;
+            int kept = 0;
+#pragma unroll
+            for (int i = 0; i < kLongList / 32; ++i) key[i] = 32 * i + lane < listed ? list[32 * i + lane] : 0ull;
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < kLongList / 32; ++i) {
+              const unsigned m = __ballot_sync(0xffffffffu, key[i] >= least);
+              if (key[i] >= least) list[kept + __popc(m & ((1u << lane) - 1))] = key[i];
+              kept += __popc(m);
+            }
+            listed = kept;
+            __syncwarp();
+          } else {  // many alike: the highest key below the last one found, topk times
+            unsigned long long below = ~0ull;
+#pragma unroll 1
+            for (int k = 0; k < p.topk; ++k) {
+              unsigned long long most = 0;
+#pragma unroll 1
+              for (int u = 1 + lane; u < p.classes + kLongEntries; u += 32) {
+                const bool dense = u < p.classes;
+                const int e = u - p.classes;
+                if (!dense && e >= n) break;
+                const int cl = dense ? u : at[e];
+                if (cl == 0 || (dense && add[cl] == -INFINITY)) continue;
+                const float y = dense ? __fadd_rn(load_logit(z + cl), add[cl])
+                                      : __fadd_rn(penalised(load_logit(z + cl), less[e], l.repeat), plus[e]);
+                const unsigned long long key1 = y > -INFINITY ? class_key(y, cl) : 0ull;
+                if (key1 < below && key1 > most) most = key1;
+              }
+              below = warp_max_key(most);
+              if (lane == 0) list[k] = below;
+            }
+            listed = p.topk;
+            __syncwarp();
+          }
+#pragma unroll
+          for (int i = 0; i < kLongList / 32; ++i) key[i] = 32 * i + lane < listed ? list[32 * i + lane] : 0ull;
+          int rank[kLongList / 32] = {};
+#pragma unroll 2
+          for (int u = 0; u < listed; ++u) {
+            const unsigned long long k = list[u];
+#pragma unroll
+            for (int i = 0; i < kLongList / 32; ++i) rank[i] += k > key[i];
+          }
+#pragma unroll
+          for (int i = 0; i < kLongList / 32; ++i)
+            if (key[i] && rank[i] < p.topk) {
+              p.ids[o + rank[i]] = static_cast<int32_t>(0xffffffffu - static_cast<uint32_t>(key[i]));
+              p.probs[o + rank[i]] = __fsub_rn(__fsub_rn(order_float(static_cast<uint32_t>(key[i] >> 32)), from.best), ln);
+            }
+          if (lane >= listed && lane < p.topk) {
+            p.ids[o + lane] = -1;
+            p.probs[o + lane] = -INFINITY;
+          }
+          __syncwarp();
+        }
+        if (lane == 0) p.blank[row] = __fsub_rn(__fsub_rn(blank, from.best), ln);
+      }
+    }
+    copy_wait_all();
+    r = end;
   }
 }
 

@@ -353,6 +353,39 @@ def test_a_history_that_names_every_class(classes, half):
         assert np.array_equal(c.keep[0].cpu().numpy().reshape(-1, classes), c.want.astype(c.z.dtype), equal_nan=True)
 
 
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("classes,pitch", [(1030, 1030), (1500, 1501), (4096, 4096), (12000, 12000), (16384, 16390)])
+def test_long_rows_in_long_lines(classes, pitch, half):
+    """Rows past what a warp holds at once, many of them a line: ties, histories that fit and that do not,
+    NaN where the rules forbid, a line behind the first block's."""
+    rng = np.random.default_rng(classes + half)
+    lengths = [33, 0, 1, 70, 18, 40]
+    at = line_places(rng, lengths, 2)
+    z = logits_of(rng, at[-1] + 3, classes, half, grid=classes == 4096)
+    rules = some_rules(rng, 6, classes, longest=200)
+    h = [rules["history"][rules["history_at"][i]:rules["history_at"][i + 1]] for i in range(6)]
+    h[4] = rng.permutation(classes)[:700].astype(np.int32)
+    h[5] = np.concatenate([[0, 0, 0], h[5], h[5]]).astype(np.int32)
+    rules["history"] = np.concatenate(h)
+    rules["history_at"] = np.concatenate([[0], np.cumsum([len(x) for x in h])]).astype(np.int32)
+    c = Case(z, at, rules, pitch)
+    c.check_greedy()
+    for k in (0, 1, 16):
+        c.check_candidates(k)
+    bad = rng.random(classes) < 0.2
+    bad[:4] = False
+    z[:, bad] = rng.choice(np.array([np.nan, np.inf], z.dtype), (len(z), bad.sum()))
+    z[40, :] = 0.5
+    z[41, 1:] = -np.inf
+    z[42, 0] = -1200
+    rules = {"bias": np.where(bad, -np.inf, 0.0).astype(np.float32)[None]}
+    c = Case(z, at, rules, pitch)
+    c.check_greedy()
+    c.check_candidates(7)
+    c = Case(z[:, :classes], at, {"bias": np.where(np.arange(classes) == 0, 0, -np.inf).astype(np.float32)[None]}, pitch)
+    c.check_candidates(2)  # nothing but the blank
+
+
 def test_the_types_lowest_value_everywhere():
     """Rows of the lowest value, as callers mask: a maximum that times log2 e overflows."""
     z = np.full((4, 900), np.finfo(np.float32).min, np.float32)
