@@ -96,6 +96,7 @@ const char* rules_fault(const crec_rules* r) {
 LineParams line_params(const crec_line_logits* z, const crec_rules* r) {
   LineParams p{};
   p.z = z->logits;
+  p.z_end = static_cast<const uint8_t*>(z->logits) + (z->rows > 0 ? ((z->rows - 1) * z->pitch + z->classes) * type_bytes(z->type) : 0);
   p.pitch = z->pitch;
   p.classes = z->classes;
   p.rows = static_cast<int>(z->rows);
@@ -188,9 +189,11 @@ cudaError_t decode(LineParams& p, cudaStream_t s) {
   else return decode_fit<kOp, T, V>(p, need, sms, s, std::integer_sequence<int, 4, 16, 32>{});
 }
 
-// Long rows where lines are long too: a block sets a line's rules for 16 warps, so from 16 frames a line
-// on average (fewer leave warps idle and pay the rules more often than a team of 16 does).
-constexpr int kLongLines = 16;
+// Long rows where lines are long too: a block sets a line's rules for 8 or 16 warps, so from 16 frames a
+// line on average (fewer leave warps idle and pay the rules more often than a team does: 140 us against
+// 105 at 8 and 30 frames a line of 12,000 classes), and from 2,048 classes (1,500: 227 us against a team's
+// 204; 2,900: 192 against 209; 12,000: 85 against 127).
+constexpr int kLongLines = 16, kLongClasses = 2048;
 
 template <int kOp, typename T, int V>
 cudaError_t decode_long(LineParams& p, cudaStream_t s) {
@@ -199,9 +202,13 @@ cudaError_t decode_long(LineParams& p, cudaStream_t s) {
   const cudaError_t e = sm_count(&sms);
   if (e != cudaSuccess) return e;
   const int chunks = (p.classes + L::kChunk - 1) / L::kChunk;
-  p.team_rows = (p.rows + sms - 1) / sms;
-  const size_t smem = sizeof(TeamRow) + kLongEntries * 10 + static_cast<size_t>(chunks) * L::kChunk * 4 + kMaxTeam * L::kWarp;
-  return launch_on(long_rows_kernel<kOp, T, V>, p, (p.rows + p.team_rows - 1) / p.team_rows, 32 * kMaxTeam, smem, s);
+  const size_t rules = sizeof(TeamRow) + kLongEntries * 10 + static_cast<size_t>(chunks) * L::kChunk * 4;
+  // Two blocks of 8 warps an SM, one at work while the other sets rules, or one of 16, whose rules serve
+  // twice the rows: the first up to 8,192 classes (12,000: 104 us against 85; 2,900: 192 against 209).
+  p.warps = p.classes <= 8192 ? kMaxTeam / 2 : kMaxTeam;
+  const int blocks = sms * (kMaxTeam / p.warps);
+  p.team_rows = (p.rows + blocks - 1) / blocks;
+  return launch_on(long_rows_kernel<kOp, T, V>, p, (p.rows + p.team_rows - 1) / p.team_rows, 32 * p.warps, rules + p.warps * L::kWarp, s);
 }
 
 template <int kOp, typename T>
@@ -241,7 +248,7 @@ template <int kOp>
 cudaError_t launch_decode(LineParams& p, int type, cudaStream_t s) {
   bias_reads(p);
   if (p.classes > kRegisterClasses) return type == CREC_FP16 ? decode_wide<kOp, __half>(p, s) : decode_wide<kOp, float>(p, s);
-  if (p.classes > 32 * kDecodeLane && p.rows / p.lines >= kLongLines) {
+  if (p.classes > kLongClasses && p.rows / p.lines >= kLongLines) {
     if (type == CREC_FP16) return wide(p.z, p.pitch, 2, 16) ? decode_long<kOp, __half, 8>(p, s) : decode_long<kOp, __half, 1>(p, s);
     return wide(p.z, p.pitch, 4, 16) ? decode_long<kOp, float, 4>(p, s) : decode_long<kOp, float, 1>(p, s);
   }

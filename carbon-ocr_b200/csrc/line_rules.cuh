@@ -20,6 +20,7 @@ namespace crec {
 
 struct LineParams {
   const void* z;  // [rows][classes], rows `pitch` elements apart
+  const void* z_end;  // past the last row's last class
   long long pitch;
   int classes, rows, lines;
   const int32_t* line_at;
@@ -129,14 +130,28 @@ constexpr int kMaxTop = 16;
 constexpr int kShortList = 64;  // a row's candidates ranked at once
 constexpr float kLog2e = 1.44269504088896341f;
 
-// `bytes` (4, 8 or 16, both ends aligned to them) to shared memory without waiting; past `valid` zeros.
-template <int kBytes>
+// 16 bytes (both ends aligned to them) to shared memory without waiting; past `valid` bytes zeros.
 __device__ __forceinline__ void copy_async(void* shared, const void* global, int valid) {
-  if constexpr (kBytes == 16)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(shared)), "l"(global), "r"(valid) : "memory");
-  else
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(smem_u32(shared)), "l"(global), "n"(kBytes), "r"(valid)
-                 : "memory");
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(shared)), "l"(global), "r"(valid) : "memory");
+}
+// n logits from any address to shared memory without waiting, by a whole warp, in the 16-byte pieces that
+// hold them: they begin at shared[returned], what comes with them on either side is of no use.  A
+// piece that reaches past the array itself (its first or its last) goes logit by logit.
+template <typename T>
+__device__ __forceinline__ int copy_row(const LineParams& p, T* shared, const T* z, int n, int lane) {
+  const uintptr_t first = reinterpret_cast<uintptr_t>(z), end = first + static_cast<uintptr_t>(max(n, 0)) * sizeof(T), low = first & ~uintptr_t(15);
+  for (uintptr_t q = low + 16 * lane; q < end; q += 512) {
+    T* s = shared + (q - low) / sizeof(T);
+    if (q >= reinterpret_cast<uintptr_t>(p.z) && q + 16 <= reinterpret_cast<uintptr_t>(p.z_end)) {
+      copy_async(s, reinterpret_cast<const void*>(q), 16);
+    } else {
+      for (int i = 0; i < 16 / static_cast<int>(sizeof(T)); ++i) {
+        const uintptr_t at = q + i * sizeof(T);
+        if (at >= first && at < end) s[i] = *reinterpret_cast<const T*>(at);
+      }
+    }
+  }
+  return static_cast<int>((first - low) / sizeof(T));
 }
 __device__ __forceinline__ void copy_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
@@ -353,10 +368,11 @@ struct WarpRow {
   static constexpr int kLane = NV * V, kSpan = 32 * kLane;  // classes of a lane, of the warp
   static constexpr int kCap = kSpan < kMaxEntries ? kSpan : kMaxEntries;
   using Rules = SpanRules<kSpan, kCap>;
-  static constexpr int kRules = Rules::kBytes, kShared = kRules + kSpan * sizeof(T);
+  static constexpr int kRules = Rules::kBytes, kShared = kRules + kSpan * sizeof(T) + (V == 1 ? 32 : 0);
   int lane, base;  // the span's first class
   LineRule l;
   uint8_t* shared;  // SpanRules, then the rows
+  int shift;  // V = 1: where in its place the row begins
   int n;  // entries
   // The first 64 entries, two a lane, in registers: place, less, bias
   int at[2];
@@ -368,30 +384,29 @@ struct WarpRow {
     shared = shared_;
     l.first = l.end = 0;
     n = 0;
+    shift = 0;
     // places past the last class stay 0 (their add is -inf)
-    for (int k = max(0, p.classes - base) + lane; k < kSpan; k += 32) place()[k] = T(0.0f);
+    if (V > 1)
+      for (int k = max(0, p.classes - base) + lane; k < kSpan; k += 32) place()[k] = T(0.0f);
     __syncwarp();
   }
   __device__ __forceinline__ const T* row(const LineParams& p, int r) const {
     return static_cast<const T*>(p.z) + r * p.pitch + base;
   }
-  __device__ __forceinline__ T* place() const { return reinterpret_cast<T*>(shared + kRules); }
+  __device__ __forceinline__ T* place() const { return reinterpret_cast<T*>(shared + kRules) + (V == 1 ? shift : 0); }
   // Row r (where r < r1) on its way.
   __device__ __forceinline__ void fetch(const LineParams& p, int r, int r1) {
-    if (r < r1) {
-      const T* z = row(p, r) + lane * V;
+    if (r >= r1) return;
+    const T* z = row(p, r);
+    if constexpr (V == 1) {
+      shift = copy_row(p, reinterpret_cast<T*>(shared + kRules), z, min(kSpan, p.classes - base), lane);
+    } else {
+      z += lane * V;
       T* s = place() + lane * V;
       const int left = p.classes - base - lane * V;
-      if constexpr (V * sizeof(T) >= 4) {
 #pragma unroll
-        for (int j = 0; j < NV; ++j)
-          if (j * 32 * V < left)
-            copy_async<V * sizeof(T)>(s + j * 32 * V, z + j * 32 * V, min(V, left - j * 32 * V) * static_cast<int>(sizeof(T)));
-      } else {
-#pragma unroll
-        for (int j = 0; j < NV; ++j)
-          if (j * 32 * V < left) s[j * 32 * V] = z[j * 32 * V];
-      }
+      for (int j = 0; j < NV; ++j)
+        if (j * 32 * V < left) copy_async(s + j * 32 * V, z + j * 32 * V, min(V, left - j * 32 * V) * static_cast<int>(sizeof(T)));
     }
   }
   __device__ __forceinline__ void arrived() const {
@@ -413,13 +428,15 @@ struct WarpRow {
   // The dense pass.  Where a forbidden class holds NaN or +inf the sum with -inf is NaN; kCareful
   // chooses instead of adding.
   template <bool kCareful>
-  __device__ __forceinline__ void ruled(float (&v)[kLane]) const {
+  __device__ __forceinline__ void ruled(const LineParams& p, float (&v)[kLane]) const {
     const float* t = reinterpret_cast<const float*>(shared) + lane * V;
     const T* z = place() + lane * V;
+    const int left = p.classes - base - lane;  // V = 1: beyond are no logits
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       float u[V], a[V];
-      get_logits<V>(z + j * 32 * V, u);
+      if constexpr (V == 1) u[0] = j * 32 < left ? load_logit(z + j * 32) : 0.0f;
+      else get_logits<V>(z + j * 32 * V, u);
       if constexpr (V == 1) {
         a[0] = t[j * 32];
       } else {
@@ -496,7 +513,7 @@ __global__ void __launch_bounds__(kRulesThreads, 8) logit_rules_kernel(const __g
     }
     float v[Row::kLane], x[2];
     row.arrived();
-    row.template ruled<true>(v);
+    row.template ruled<true>(p, v);
     row.pair(x);
     __syncwarp();
     const bool early = row.n <= 64;  // entries past the registers' are read from the row's place below
@@ -782,7 +799,7 @@ __global__ void __launch_bounds__(32 * kMaxTeam, 1) line_rows_kernel(const __gri
     }
     float v[Row::kLane], x[2];
     row.arrived();
-    row.template ruled<false>(v);
+    row.template ruled<false>(p, v);
     row.pair(x);
     __syncwarp();
     row.fetch(p, r + 1, r1);
@@ -936,13 +953,13 @@ __global__ void __launch_bounds__(32 * kMaxTeam, 1) line_rows_kernel(const __gri
 
 // ---------------------------------------------------------------- long rows
 //
-// More than 1,024 classes, many frames a line: a warp a row all the same, a block of 16 warps a line's
-// rows.  The line's rules on all classes lie in shared memory once for the block; a row comes through
+// More than 1,024 classes, many frames a line: a warp a row all the same, a block of 8 or 16 warps
+// a line's rows.  The line's rules on all classes lie in shared memory once for the block; a row comes through
 // its warp in chunks, three places deep, with the maximum and the sum of exp(z - base) kept as it goes
 // (the base, one for the warp, rises with the maximum, and the sum is scaled by the bases' exact
 // difference).  No barrier a row: teams of 16 warps that meet twice a row took 3 times as long
 // (4,096 x 12,000 float16: 127 us).  Candidates are listed as they reach what the lanes' maxima so far
-// promise of the k-th highest, and the list is cut to what the last promise leaves before it is ranked.
+// promise of the k-th highest; a full list is cut to its k highest, and nothing below those comes in.
 
 constexpr int kLongEntries = 256;  // of a line; one with more goes the slow way
 constexpr int kLongList = 128;     // keys of a row
@@ -951,8 +968,35 @@ constexpr int kLongPlaces = 3;
 template <typename T, int V>
 struct LongRow {
   static constexpr int NV = V == 1 ? 16 : 4, kLane = NV * V, kChunk = 32 * kLane;
-  static constexpr int kWarp = kLongPlaces * kChunk * static_cast<int>(sizeof(T)) + kLongList * 8;  // shared bytes of a warp
+  static constexpr int kPlace = kChunk + (V == 1 ? 32 / static_cast<int>(sizeof(T)) : 0);  // logits a place holds
+  static constexpr int kWarp = kLongPlaces * kPlace * static_cast<int>(sizeof(T)) + kLongList * 8;  // shared bytes of a warp
 };
+
+// A warp's listed keys but the k highest dropped, those put in order at the front; the k-th (0 where
+// there are fewer).  All of them are at most kLongList.
+__device__ __noinline__ unsigned long long keep_highest(unsigned long long* list, int listed, int k) {
+  const int lane = threadIdx.x % 32;
+  __syncwarp();
+  unsigned long long key[kLongList / 32];
+  int rank[kLongList / 32];
+#pragma unroll
+  for (int i = 0; i < kLongList / 32; ++i) {
+    key[i] = 32 * i + lane < listed ? list[32 * i + lane] : 0ull;
+    rank[i] = 0;
+  }
+#pragma unroll 4
+  for (int u = 0; u < listed; ++u) {
+    const unsigned long long other = list[u];
+#pragma unroll
+    for (int i = 0; i < kLongList / 32; ++i) rank[i] += other > key[i];
+  }
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < kLongList / 32; ++i)
+    if (key[i] && rank[i] < k) list[rank[i]] = key[i];
+  __syncwarp();
+  return listed >= k ? list[k - 1] : 0ull;
+}
 
 template <int kOp, typename T, int V>
 __global__ void __launch_bounds__(32 * kMaxTeam, 1) long_rows_kernel(const __grid_constant__ LineParams p) {
@@ -969,9 +1013,9 @@ __global__ void __launch_bounds__(32 * kMaxTeam, 1) long_rows_kernel(const __gri
   float* add = reinterpret_cast<float*>(at + kLongEntries);  // [chunks * kChunk]
   uint8_t* mine = reinterpret_cast<uint8_t*>(add + chunks * L::kChunk) + w * L::kWarp;
   T* places = reinterpret_cast<T*>(mine);
-  unsigned long long* list = reinterpret_cast<unsigned long long*>(mine + kLongPlaces * L::kChunk * sizeof(T));
+  unsigned long long* list = reinterpret_cast<unsigned long long*>(mine + kLongPlaces * L::kPlace * sizeof(T));
   auto clear = [&]() {  // past the last class: 0 (its add is -inf)
-    for (int k = lane; k < kLongPlaces * L::kChunk; k += 32) places[k] = T(0.0f);
+    for (int k = lane; k < kLongPlaces * L::kPlace; k += 32) places[k] = T(0.0f);
     __syncwarp();
   };
   clear();
@@ -989,22 +1033,21 @@ __global__ void __launch_bounds__(32 * kMaxTeam, 1) long_rows_kernel(const __gri
     int f_row = r + w, f_chunk = 0, f_place = 0;
     auto fetch = [&]() {
       if (f_row < end) {
-        const int c = f_chunk * L::kChunk + lane * V;
+        const int c = f_chunk * L::kChunk;
         const T* z = static_cast<const T*>(p.z) + f_row * p.pitch + c;
-        T* s = places + f_place * L::kChunk + lane * V;
-        const int left = p.classes - c;
+        T* s = places + f_place * L::kPlace;
+        if constexpr (V == 1) {
+          copy_row(p, s, z, min(L::kChunk, p.classes - c), lane);
+        } else {
+          const int left = p.classes - c - lane * V;
 #pragma unroll
-        for (int j = 0; j < L::NV; ++j) {
-          if constexpr (V * sizeof(T) >= 4) {
+          for (int j = 0; j < L::NV; ++j)
             if (j * 32 * V < left)
-              copy_async<V * sizeof(T)>(s + j * 32 * V, z + j * 32 * V, min(V, left - j * 32 * V) * static_cast<int>(sizeof(T)));
-          } else {
-            if (j * 32 * V < left) s[j * 32 * V] = z[j * 32 * V];
-          }
+              copy_async(s + (j * 32 + lane) * V, z + (j * 32 + lane) * V, min(V, left - j * 32 * V) * static_cast<int>(sizeof(T)));
         }
         if (++f_chunk == chunks) {
           f_chunk = 0;
-          f_row += kMaxTeam;
+          f_row += p.warps;
         }
       }
       f_place = f_place + 1 == kLongPlaces ? 0 : f_place + 1;
@@ -1058,14 +1101,14 @@ __global__ void __launch_bounds__(32 * kMaxTeam, 1) long_rows_kernel(const __gri
     if (n > kLongEntries) {
       copy_wait_all();
       __syncthreads();
-      for (; r < end; ++r) slow_row<kOp, T, true>(p, r, l, t, reinterpret_cast<uint8_t*>(add) + w * SpanRules<kSlowSpan, kSlowSpan>::kBytes, w, kMaxTeam);
+      for (; r < end; ++r) slow_row<kOp, T, true>(p, r, l, t, reinterpret_cast<uint8_t*>(add) + w * SpanRules<kSlowSpan, kSlowSpan>::kBytes, w, p.warps);
       clear();  // (slow rows work in the table and in what follows it)
       continue;
     }
 
     int place = 0;
 #pragma unroll 1
-    for (int row = r + w; row < end; row += kMaxTeam) {
+    for (int row = r + w; row < end; row += p.warps) {
       const T* z = static_cast<const T*>(p.z) + row * p.pitch;
       // the entries first (at most 8 a lane); the blank apart
       float blank = -INFINITY, high = -INFINITY, x[kLongEntries / 32];
@@ -1088,10 +1131,16 @@ __global__ void __launch_bounds__(32 * kMaxTeam, 1) long_rows_kernel(const __gri
       float2 s[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
       float c = __fmul_rn(best == -INFINITY ? 0.0f : best, kLog2e);
       bool based = best > -INFINITY;  // c belongs to a logit
+      unsigned long long least = 0;  // k keys are above it
       auto push = [&](bool takes, float y, int k) {  // by whole warps
-        const unsigned m = __ballot_sync(0xffffffffu, takes);
-        const int to = listed + __popc(m & ((1u << lane) - 1));
-        if (takes && to < kLongList) list[to] = class_key(y, k);
+        const unsigned long long key = class_key(y, k);
+        unsigned m = __ballot_sync(0xffffffffu, takes && key > least);
+        if (listed + __popc(m) > kLongList) {
+          least = keep_highest(list, listed, p.topk);
+          listed = min(listed, p.topk);
+          m = __ballot_sync(0xffffffffu, takes && key > least);
+        }
+        if (m >> lane & 1) list[listed + __popc(m & ((1u << lane) - 1))] = key;
         listed += __popc(m);
       };
 #pragma unroll
@@ -1109,11 +1158,14 @@ __global__ void __launch_bounds__(32 * kMaxTeam, 1) long_rows_kernel(const __gri
         __syncwarp();
         float v[L::kLane];
         const float* a = add + chunk * L::kChunk + lane * V;
-        const T* q = places + place * L::kChunk + lane * V;
+        const int shift = V == 1 ? static_cast<int>(reinterpret_cast<uintptr_t>(z) % 16 / sizeof(T)) : 0;  // as copy_row leaves it
+        const T* q = places + place * L::kPlace + shift + lane * V;
+        const int left = p.classes - chunk * L::kChunk - lane;
 #pragma unroll
         for (int j = 0; j < L::NV; ++j) {
           float u[V];
-          get_logits<V>(q + j * 32 * V, u);
+          if constexpr (V == 1) u[0] = j * 32 < left ? load_logit(q + j * 32) : 0.0f;
+          else get_logits<V>(q + j * 32 * V, u);
           if constexpr (V == 1) {
             v[j] = __fadd_rn(u[0], a[j * 32]);
           } else {
@@ -1182,7 +1234,7 @@ __global__ void __launch_bounds__(32 * kMaxTeam, 1) long_rows_kernel(const __gri
             }
             while (__any_sync(0xffffffffu, bits != 0)) {  // a lane's lowest at a time, read again from its place
               const int i = max(__ffs(bits) - 1, 0), k = (i / V * 32 + lane) * V + i % V;
-              push(bits != 0, __fadd_rn(load_logit(places + place * L::kChunk + k), add[chunk * L::kChunk + k]), chunk * L::kChunk + k);
+              push(bits != 0, __fadd_rn(load_logit(places + place * L::kPlace + shift + k), add[chunk * L::kChunk + k]), chunk * L::kChunk + k);
               bits &= bits - 1;
             }
           }
@@ -1225,68 +1277,15 @@ __global__ void __launch_bounds__(32 * kMaxTeam, 1) long_rows_kernel(const __gri
         const float ln = some ? logf(__fdiv_rn(sum, from.term(from.best))) : sum;
         const size_t o = static_cast<size_t>(row) * p.topk;
         if (p.topk > 0) {
-          __syncwarp();
-          unsigned long long key[kLongList / 32];  // what the last promise leaves, moved to the front
           reach = kth_group(high, p.topk, lane);
 #pragma unroll
           for (int i = 0; i < kLongEntries / 32; ++i)
             if (32 * i < n) push(x[i] >= reach, x[i], 32 * i + lane < n ? at[32 * i + lane] : 0);
-          __syncwarp();
-          if (listed <= kLongList) {
-            const unsigned long long least = static_cast<unsigned long long>(float_order(reach)) << 32;
-            int kept = 0;
-#pragma unroll
-            for (int i = 0; i < kLongList / 32; ++i) key[i] = 32 * i + lane < listed ? list[32 * i + lane] : 0ull;
-            __syncwarp();
-#pragma unroll
-            for (int i = 0; i < kLongList / 32; ++i) {
-              const unsigned m = __ballot_sync(0xffffffffu, key[i] >= least);
-              if (key[i] >= least) list[kept + __popc(m & ((1u << lane) - 1))] = key[i];
-              kept += __popc(m);
-            }
-            listed = kept;
-            __syncwarp();
-          } else {  // many alike: the highest key below the last one found, topk times
-            unsigned long long below = ~0ull;
-#pragma unroll 1
-            for (int k = 0; k < p.topk; ++k) {
-              unsigned long long most = 0;
-#pragma unroll 1
-              for (int u = 1 + lane; u < p.classes + kLongEntries; u += 32) {
-                const bool dense = u < p.classes;
-                const int e = u - p.classes;
-                if (!dense && e >= n) break;
-                const int cl = dense ? u : at[e];
-                if (cl == 0 || (dense && add[cl] == -INFINITY)) continue;
-                const float y = dense ? __fadd_rn(load_logit(z + cl), add[cl])
-                                      : __fadd_rn(penalised(load_logit(z + cl), less[e], l.repeat), plus[e]);
-                const unsigned long long key1 = y > -INFINITY ? class_key(y, cl) : 0ull;
-                if (key1 < below && key1 > most) most = key1;
-              }
-              below = warp_max_key(most);
-              if (lane == 0) list[k] = below;
-            }
-            listed = p.topk;
-            __syncwarp();
-          }
-#pragma unroll
-          for (int i = 0; i < kLongList / 32; ++i) key[i] = 32 * i + lane < listed ? list[32 * i + lane] : 0ull;
-          int rank[kLongList / 32] = {};
-#pragma unroll 2
-          for (int u = 0; u < listed; ++u) {
-            const unsigned long long k = list[u];
-#pragma unroll
-            for (int i = 0; i < kLongList / 32; ++i) rank[i] += k > key[i];
-          }
-#pragma unroll
-          for (int i = 0; i < kLongList / 32; ++i)
-            if (key[i] && rank[i] < p.topk) {
-              p.ids[o + rank[i]] = static_cast<int32_t>(0xffffffffu - static_cast<uint32_t>(key[i]));
-              p.probs[o + rank[i]] = __fsub_rn(__fsub_rn(order_float(static_cast<uint32_t>(key[i] >> 32)), from.best), ln);
-            }
-          if (lane >= listed && lane < p.topk) {
-            p.ids[o + lane] = -1;
-            p.probs[o + lane] = -INFINITY;
+          keep_highest(list, listed, p.topk);
+          if (lane < p.topk) {
+            const unsigned long long key = lane < listed ? list[lane] : 0ull;
+            p.ids[o + lane] = key ? static_cast<int32_t>(0xffffffffu - static_cast<uint32_t>(key)) : -1;
+            p.probs[o + lane] = key ? __fsub_rn(__fsub_rn(order_float(static_cast<uint32_t>(key >> 32)), from.best), ln) : -INFINITY;
           }
           __syncwarp();
         }
