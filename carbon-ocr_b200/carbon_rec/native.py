@@ -29,7 +29,7 @@ EXPORTS = ["crec_open", "crec_close", "crec_last_error", "crec_is_broken", "crec
            "crec_stream", "crec_debug_crops", "crec_debug_value", "crec_debug_logits", "crec_last_stats", "crec_candidates",
            "crec_profile", "crec_profile_layers", "crec_mma_peak", "crec_debug_inject", "crec_conv_sweep",
            "crec_head_sweep", "crec_ctc_head_blob", "crec_logit_rules", "crec_ctc_greedy_lines", "crec_candidates_lines",
-           "crec_blob_head", "crec_adapters_open", "crec_adapters_close", "crec_adapters_logits"]
+           "crec_head_input", "crec_blob_head", "crec_adapters_open", "crec_adapters_close", "crec_adapters_logits"]
 
 
 class CrecError(RuntimeError):
@@ -129,6 +129,7 @@ def lib() -> C.CDLL:
         L.crec_debug_logits.argtypes = [p, p, i64]
         L.crec_last_stats.argtypes = [p, C.POINTER(Stats)]
         L.crec_candidates.argtypes = [p, p, i, i, p, p, p, p, p, i64]
+        L.crec_head_input.argtypes = [p, p, i, p, p, i64, i64]
         L.crec_profile.argtypes = [p, i, C.POINTER(ProfileEntry), i]
         L.crec_profile_layers.argtypes = [p, C.POINTER(ProfileEntry), i]
         L.crec_mma_peak.argtypes = [i, i, i, i, C.POINTER(C.c_double)]
@@ -598,6 +599,15 @@ class RecDevice:
                         blank[at:at + t]))
             at += t
         return out
+
+    def head_input(self, rows, x_ptr: int, pitch: int, capacity: int) -> np.ndarray:
+        """crec_head_input: the head's input of lines `rows` of the last recognize call into x (a device address,
+        float16, frames `pitch` elements apart); line_at [n + 1], each line's first frame in x."""
+        rows = np.ascontiguousarray(rows, np.int32)
+        line_at = np.zeros(len(rows) + 1, np.int32)
+        self._check(lib().crec_head_input(self._h, rows.ctypes.data, len(rows), line_at.ctypes.data, x_ptr or None, int(pitch),
+                                          int(capacity)))
+        return line_at
 
     def value(self, index: int, nbytes: int, dtype=np.uint8) -> np.ndarray:
         out = np.zeros(nbytes, np.uint8)

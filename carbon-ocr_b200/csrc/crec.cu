@@ -277,6 +277,8 @@ struct crec_handle {
   std::vector<int> last_frame0, last_len;  // its lines' first frame columns and lengths (the beam's candidates)
   // crec_candidates' buffers (grown on demand)
   int32_t* d_cand_cols = nullptr;
+  int32_t* d_input_cols = nullptr;  // crec_head_input's
+  size_t cap_input_cols = 0;
   int32_t* d_cand_ids = nullptr;
   float* d_cand_vals = nullptr;
   float* d_cand_fr = nullptr;  // [3][frames]: best, sum, the blank's logit
@@ -1689,6 +1691,7 @@ void free_all(crec_handle* h) {
   cudaFree(h->d_order);
   cudaFreeHost(h->hs_order);
   cudaFree(h->d_cand_cols);
+  cudaFree(h->d_input_cols);
   cudaFree(h->d_cand_ids);
   cudaFree(h->d_cand_vals);
   cudaFree(h->d_cand_fr);
@@ -2417,6 +2420,43 @@ int crec_candidates(crec_handle* h, const int32_t* rows, int n, int topk, int32_
     blank[f] = fr[2 * total + f] - off;
   }
   return CREC_OK;
+}
+
+int crec_head_input(crec_handle* h, const int32_t* rows, int n, int32_t* line_at, void* x, int64_t pitch, int64_t capacity) try {
+  if (!h) return CREC_E_INVALID;
+  if (h->broken) return set_error(h, CREC_E_STICKY, "the GPU is broken for this process");
+  if (n < 0 || !line_at || (n > 0 && !rows)) return set_error(h, CREC_E_INVALID, "head_input: arguments");
+  const Layer& head = h->l.back();
+  const Value& v = h->v[head.in];
+  const Value& vp = h->v[v.phys];
+  if (pitch < v.c) return set_error(h, CREC_E_INVALID, "head_input: a pitch of at least the head's channels");
+  std::vector<int32_t> cols;
+  line_at[0] = 0;
+  for (int j = 0; j < n; ++j) {
+    const int r = rows[j] - h->last_a;
+    if (r < 0 || r >= h->last_n)
+      return set_error(h, CREC_E_RANGE, "head_input: line " + std::to_string(rows[j]) +
+                                            " is not in the last run of the last recognize call");
+    for (int t = 0; t < h->last_len[r]; ++t) cols.push_back(h->last_frame0[r] + t);
+    line_at[j + 1] = static_cast<int32_t>(cols.size());
+  }
+  const size_t total = cols.size();
+  if (static_cast<int64_t>(total) > capacity) return set_error(h, CREC_E_RANGE, "head_input: capacity too small");
+  if (total == 0) return CREC_OK;
+  if (!x || reinterpret_cast<uintptr_t>(x) % 2) return set_error(h, CREC_E_INVALID, "head_input: no x");
+  CK(cudaSetDevice(h->device));
+  int rc;
+  if ((rc = grow_device(h, &h->d_input_cols, &h->cap_input_cols, total))) return rc;
+  CK(cudaMemcpyAsync(h->d_input_cols, cols.data(), sizeof(int32_t) * total, cudaMemcpyHostToDevice, h->stream));
+  auto* k = h->int8 ? head_input_kernel<true> : head_input_kernel<false>;
+  k<<<static_cast<unsigned>((total + 3) / 4), 128, 0, h->stream>>>(vp.base + static_cast<long long>(vp.ph) * vp.pitch, v.cp, v.c, v.zero,
+                                                                   v.scale, h->d_input_cols, static_cast<int>(total),
+                                                                   static_cast<__half*>(x), pitch);
+  CK(cudaGetLastError());
+  CK(cudaStreamSynchronize(h->stream));
+  return CREC_OK;
+} catch (const std::bad_alloc&) {
+  return set_error(h, CREC_E_NOMEM, "head_input: host memory");
 }
 
 int crec_last_stats(const crec_handle* h, crec_stats* out) {

@@ -90,6 +90,21 @@ struct CandParams {
   float* blank;        // [frames] the blank's logit
 };
 
+// The head's input of frames of the last run, as float16 rows for a head of the caller's own: a warp a
+// frame, INT8 codes as (code - zero) * scale rounded once.
+template <bool kInt8>
+__global__ void __launch_bounds__(128) head_input_kernel(const uint8_t* x, int cp, int k, int zero, float scale, const int32_t* cols,
+                                                         int frames, __half* out, long long pitch) {
+  const int f = blockIdx.x * 4 + threadIdx.x / 32;
+  if (f >= frames) return;
+  const uint8_t* src = x + static_cast<long long>(cols[f]) * cp * (kInt8 ? 1 : 2);
+  __half* o = out + f * pitch;
+  for (int c = threadIdx.x % 32; c < k; c += 32) {
+    if constexpr (kInt8) o[c] = __float2half_rn(__fmul_rn(static_cast<float>(static_cast<int>(src[c]) - zero), scale));
+    else o[c] = reinterpret_cast<const __half*>(src)[c];
+  }
+}
+
 constexpr int kCandThreads = 256;
 
 // One CTA a frame: the frame's channels into shared memory, a thread a class's logit (INT8: the

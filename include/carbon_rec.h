@@ -195,6 +195,14 @@ CREC_API int crec_crop_region(const crec_box* box, const crec_crop_rule* rule, d
 CREC_API int crec_candidates(crec_handle* h, const int32_t* rows, int n, int topk, int32_t* k, int32_t* frames,
                              int32_t* ids, float* logp, float* blank, int64_t capacity);
 
+/* The head's input of lines rows[0..n) of the last recognize call (as crec_candidates takes them),
+ * for a head of the caller's own beside it (crec_adapters_logits): the lines' frames end to end, frame
+ * f's channels at x + f * pitch, float16 on this handle's GPU (INT8: the codes' values, rounded),
+ * line j's frames [line_at[j], line_at[j + 1]) (line_at [n + 1], host).  capacity: the frames x holds;
+ * pitch in elements, at least the head's channels.  Waited for.  No counterpart in the reference. */
+CREC_API int crec_head_input(crec_handle* h, const int32_t* rows, int n, int32_t* line_at, void* x, int64_t pitch,
+                             int64_t capacity);
+
 /* What the last call did: device runs, kernel launches, bytes copied host -> device and back
  * (for crec_set_pages, the upload of the pages it took, whether it made that upload itself or a
  * crec_prefetch_pages made it); and the bytes copied each way since the handle was opened (every
