@@ -10,6 +10,7 @@ fallback: without it, or without a B200, opening a device raises.
 from __future__ import annotations
 
 import ctypes as C
+import threading
 from dataclasses import dataclass
 from pathlib import Path
 
@@ -29,7 +30,8 @@ EXPORTS = ["crec_open", "crec_close", "crec_last_error", "crec_is_broken", "crec
            "crec_stream", "crec_debug_crops", "crec_debug_value", "crec_debug_logits", "crec_last_stats", "crec_candidates",
            "crec_profile", "crec_profile_layers", "crec_mma_peak", "crec_debug_inject", "crec_conv_sweep",
            "crec_head_sweep", "crec_ctc_head_blob", "crec_logit_rules", "crec_ctc_greedy_lines", "crec_candidates_lines",
-           "crec_head_input", "crec_blob_head", "crec_adapters_open", "crec_adapters_close", "crec_adapters_logits"]
+           "crec_head_input", "crec_blob_head", "crec_adapters_open", "crec_adapters_close", "crec_adapters_logits",
+           "crec_adapters_inject"]
 
 
 class CrecError(RuntimeError):
@@ -144,6 +146,7 @@ def lib() -> C.CDLL:
         L.crec_blob_head.argtypes = [p, C.c_size_t, C.POINTER(i), C.POINTER(i), C.c_char_p, C.c_size_t]
         L.crec_adapters_open.argtypes = [i, p, C.c_size_t, i, p, p, p, p, C.POINTER(p), C.c_char_p, C.c_size_t]
         L.crec_adapters_close.argtypes = [p]
+        L.crec_adapters_inject.argtypes = [p]
         L.crec_adapters_logits.argtypes = [p, p, i64, i64, i, p, p, p, i, i64, *e]
         _lib = L
     return _lib
@@ -183,6 +186,16 @@ def ctc_greedy_noalloc(logits_ptr: int, n: int, classes: int, frames: int, lengt
         raise CrecError(rc, err.value.decode())
 
 
+class _Errors(threading.local):
+    """Each thread's buffer for the calls' messages."""
+
+    def __init__(self):
+        self.text = C.create_string_buffer(256)
+
+
+_errors = _Errors()
+
+
 def _raise(rc: int, err) -> None:
     raise CrecError(rc, err.value.decode())
 
@@ -191,9 +204,8 @@ def logit_rules(frames: LineLogits, rules: Rules | None, out_ptr: int, out_type:
                 stream: int = 0) -> None:
     """crec_logit_rules: the frames' logits under their lines' rules into out (out_pitch 0: the classes);
     queued on `stream`, not waited for."""
-    err = C.create_string_buffer(256)
-    rc = lib().crec_logit_rules(C.byref(frames), C.byref(rules) if rules is not None else None, out_ptr, out_type,
-                                out_pitch or frames.classes, stream or None, err, 256)
+    err = _errors.text
+    rc = (_lib or lib()).crec_logit_rules(frames, rules, out_ptr, out_type, out_pitch or frames.classes, stream or None, err, 256)
     if rc != OK:
         _raise(rc, err)
 
@@ -202,9 +214,8 @@ def ctc_greedy_lines(frames: LineLogits, rules: Rules | None, counts_ptr: int, i
                      probs_ptr: int, stream: int = 0) -> None:
     """crec_ctc_greedy_lines: greedy CTC of packed lines under their rules, every pointer a device address;
     queued on `stream`, not waited for."""
-    err = C.create_string_buffer(256)
-    rc = lib().crec_ctc_greedy_lines(C.byref(frames), C.byref(rules) if rules is not None else None, counts_ptr,
-                                     ids_ptr, starts_ptr, probs_ptr, stream or None, err, 256)
+    err = _errors.text
+    rc = (_lib or lib()).crec_ctc_greedy_lines(frames, rules, counts_ptr, ids_ptr, starts_ptr, probs_ptr, stream or None, err, 256)
     if rc != OK:
         _raise(rc, err)
 
@@ -213,9 +224,8 @@ def candidates_lines(frames: LineLogits, rules: Rules | None, topk: int, ids_ptr
                      stream: int = 0) -> None:
     """crec_candidates_lines: each frame's topk likeliest classes but the blank under its line's rules, every
     pointer a device address; queued on `stream`, not waited for."""
-    err = C.create_string_buffer(256)
-    rc = lib().crec_candidates_lines(C.byref(frames), C.byref(rules) if rules is not None else None, topk, ids_ptr,
-                                     logp_ptr, blank_ptr, stream or None, err, 256)
+    err = _errors.text
+    rc = (_lib or lib()).crec_candidates_lines(frames, rules, topk, ids_ptr, logp_ptr, blank_ptr, stream or None, err, 256)
     if rc != OK:
         _raise(rc, err)
 
@@ -251,11 +261,15 @@ class Adapters:
         (pitches 0: K and the classes); queued on `stream`, not waited for."""
         if not self._h:
             raise CrecError(E_INVALID, "the adapters are closed")
-        err = C.create_string_buffer(256)
-        rc = lib().crec_adapters_logits(self._h, x_ptr, x_pitch or self.k, rows, lines, line_at_ptr, adapter_ptr or None,
-                                        logits_ptr, type, pitch or self.classes, stream or None, err, 256)
+        err = _errors.text
+        rc = (_lib or lib()).crec_adapters_logits(self._h, x_ptr, x_pitch or self.k, rows, lines, line_at_ptr, adapter_ptr or None,
+                                                  logits_ptr, type, pitch or self.classes, stream or None, err, 256)
         if rc != OK:
             _raise(rc, err)
+
+    def inject(self) -> None:
+        """Test hook: the next launch's waits run out (crec_adapters_inject)."""
+        lib().crec_adapters_inject(self._h)
 
     def close(self) -> None:
         if getattr(self, "_h", None):

@@ -58,7 +58,8 @@ struct AdapterParams {
   int stages;
   uint32_t stage_bytes, h_bytes;  // h_bytes: of one of h's two words
   int* err;
-  unsigned long long wait_ns;
+  unsigned long long wait_ns;  // every wait's limit (kWaitNs; shorter only for a test's injected timeout)
+  int idle;                    // that test: nothing is loaded
 };
 
 // What the roles of a block know of a tile's frames.
@@ -320,7 +321,7 @@ __global__ void __launch_bounds__(kAdapterThreads, 1) adapter_head_kernel(const 
     // ---------------------------------------------------------------- loads
     const bool leader = elect_one();
     uint32_t g = 0, st = 0, phase = 1, q = 0;  // stages issued, the next one and its phase, chunks
-    bool ok = true;
+    bool ok = p.idle == 0;
     auto stage = [&](uint32_t bytes) -> int {  // the next stage, empty, expecting `bytes`
       const int i = st;
       ok = mbar_wait_warp(&s.empty[i], phase, p.err, kErrTimeoutEmpty, p.wait_ns);

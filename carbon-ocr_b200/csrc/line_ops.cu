@@ -295,6 +295,7 @@ struct crec_adapters {
   __half* a = nullptr;   // [adapters][r16][k]
   float* b = nullptr;    // [adapters][classes][rank]
   float* scale = nullptr;
+  std::atomic<bool> inject{false};  // the next launch's waits run out (crec_adapters_inject)
   int* err = nullptr;  // pinned, written by a launch whose bounded wait ran out
 };
 
@@ -631,6 +632,12 @@ int crec_adapters_close(crec_adapters* h) {
   return rc;
 }
 
+int crec_adapters_inject(crec_adapters* h) {
+  if (!h) return CREC_E_INVALID;
+  h->inject = true;
+  return CREC_OK;
+}
+
 int crec_adapters_logits(crec_adapters* h, const void* x, int64_t x_pitch, int64_t rows, int lines,
                          const int32_t* line_at, const int32_t* adapter, void* logits, int type, int64_t pitch,
                          void* stream, char* error, size_t error_size) {
@@ -662,7 +669,8 @@ int crec_adapters_logits(crec_adapters* h, const void* x, int64_t x_pitch, int64
   const size_t element = type_bytes(type);
   p.width = wide(logits, pitch, element, 32) ? 32 : wide(logits, pitch, element, 16) ? 16 : static_cast<int>(element);
   p.err = h->err;
-  p.wait_ns = kWaitNs;
+  p.idle = h->inject.exchange(false);
+  p.wait_ns = p.idle ? 1000000ull : kWaitNs;
   plan_adapters(h, &p);
   bool maps = encode(&p.x, x, true, h->k, p.rows, 1, x_pitch, 64, p.tile_rows) && encode(&p.w, h->w, true, h->k, h->classes, 1, h->k, 64, p.n);
   if (maps && h->adapters)

@@ -392,6 +392,9 @@ CREC_API int crec_adapters_close(crec_adapters* h);
 CREC_API int crec_adapters_logits(crec_adapters* h, const void* x, int64_t x_pitch, int64_t rows, int lines,
                                   const int32_t* line_at, const int32_t* adapter, void* logits, int type,
                                   int64_t pitch, void* stream, char* error, size_t error_size);
+/* Test hook: the next crec_adapters_logits launch loads nothing and its waits give up after 1 ms
+ * (as crec_debug_inject's CREC_INJECT_TIMEOUT): it ends, and later calls report CREC_E_TIMEOUT. */
+CREC_API int crec_adapters_inject(crec_adapters* h);
 
 /* The CUDA stream (a cudaStream_t) the handle's work runs on, for device-side timing. */
 CREC_API void* crec_stream(crec_handle* h);

@@ -162,6 +162,26 @@ def test_streams_graphs_and_two_calls_at_once():
     a.check(out)
 
 
+def test_a_wait_that_runs_out_ends_the_launch():
+    """Nothing loaded: the launch ends, the calls after it say so, and the GPU and other handles go on."""
+    import torch
+    for lengths in (LENGTHS, [100] * 400):
+        c = Case(256, 800, [16, 8], lengths)
+        c.upload()
+        h = c.open()
+        c.check(c.queue(h))
+        h.inject()
+        c.queue(h)
+        torch.cuda.synchronize()
+        for call in (lambda: c.queue(h), h.close):
+            with pytest.raises(native.CrecError) as e:
+                call()
+            assert e.value.code == native.E_TIMEOUT
+        h = c.open()
+        c.check(c.queue(h))
+        h.close()
+
+
 def test_the_same_bits_every_time():
     import torch
     c = Case(192, 1500, [16] * 8, [30] * 40)
