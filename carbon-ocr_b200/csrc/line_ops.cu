@@ -10,6 +10,7 @@
 #include <cstdint>
 #include <cstdio>
 #include <cstring>
+#include <initializer_list>
 #include <memory>
 #include <new>
 #include <string>
@@ -32,6 +33,7 @@ struct Errors {
     return code;
   }
   int cuda(cudaError_t e, const char* what) const {
+    cudaGetLastError();  // told here: not the next call's
     char msg[256];
     std::snprintf(msg, sizeof msg, "%s: %s", what, cudaGetErrorString(e));
     return (*this)(e == cudaErrorMemoryAllocation ? CREC_E_NOMEM : CREC_E_CUDA, msg);
@@ -68,8 +70,18 @@ class OnDeviceOf {
 
 size_t type_bytes(int type) { return type == CREC_FP16 ? 2 : 4; }
 bool is_logits_type(int type) { return type == CREC_FP32 || type == CREC_FP16; }
-constexpr int64_t kMaxRows = 0x7fffffff;
-constexpr int64_t kMaxPitch = int64_t{1} << 40;
+constexpr int64_t kMaxRows = 0x7fffff00;  // a tile past them still counts in 32 bits
+
+// Whether an array of `rows` rows has such a pitch (its bytes far within 64 bits).
+bool fits_pitch(int64_t pitch, int64_t least, int64_t rows) {
+  return pitch >= least && pitch <= (int64_t{1} << 40) && pitch <= (int64_t{1} << 60) / std::max<int64_t>(rows, 1);
+}
+// Whether every array is one of 4-byte values by its address (null ones too).
+bool aligned4(std::initializer_list<const void*> arrays) {
+  uintptr_t bits = 0;
+  for (const void* a : arrays) bits |= reinterpret_cast<uintptr_t>(a);
+  return bits % 4 == 0;
+}
 
 // What every call on packed lines checks; null where it passes.
 const char* lines_fault(const crec_line_logits* z) {
@@ -77,7 +89,8 @@ const char* lines_fault(const crec_line_logits* z) {
   if (!is_logits_type(z->type)) return "the logits' type";
   if (z->classes < 1 || z->classes > kMaxClasses) return "classes";
   if (z->rows < 0 || z->rows > kMaxRows || z->lines < 0) return "rows or lines";
-  if (z->pitch < z->classes || z->pitch > kMaxPitch) return "pitch";
+  if (!fits_pitch(z->pitch, z->classes, z->rows)) return "pitch";
+  if (!aligned4({z->line_at})) return "line_at's alignment";
   if (z->lines > 0 && !z->line_at) return "no line_at";
   if (z->lines > 0 && z->rows > 0 && !z->logits) return "no logits";
   if (reinterpret_cast<uintptr_t>(z->logits) % type_bytes(z->type)) return "the logits' alignment";
@@ -90,6 +103,8 @@ const char* rules_fault(const crec_rules* r) {
   if (!r->history && (r->repeat || r->presence || r->frequency)) return "penalties without a history";
   if (r->bias ? r->biases < 1 : r->bias_of != nullptr) return "bias tables";
   if (r->allowed ? r->sets < 1 : r->set_of != nullptr) return "allowed sets";
+  if (!aligned4({r->history, r->history_at, r->repeat, r->presence, r->frequency, r->bias, r->bias_of, r->allowed, r->set_of}))
+    return "the rules' alignment";
   return nullptr;
 }
 
@@ -486,7 +501,6 @@ int open_adapters(int device, const void* model, size_t model_bytes, int n, cons
   OnDeviceOf on;
   cudaError_t e = on.to(device);
   if (e != cudaSuccess) {
-    cudaGetLastError();
     return fail.cuda(e, "adapters_open");
   }
   int major = 0;
@@ -510,7 +524,6 @@ int open_adapters(int device, const void* model, size_t model_bytes, int n, cons
   if (e == cudaSuccess)
     e = cudaFuncSetAttribute(adapter_head_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448);
   if (e != cudaSuccess) {
-    cudaGetLastError();
     return fail.cuda(e, "adapters_open");
   }
   *out = h.release();
@@ -527,7 +540,7 @@ int crec_logit_rules(const crec_line_logits* z, const crec_rules* rules, void* o
   if (const char* m = lines_fault(z)) return fail(CREC_E_INVALID, m);
   if (const char* m = rules_fault(rules)) return fail(CREC_E_INVALID, m);
   if (!is_logits_type(out_type)) return fail(CREC_E_INVALID, "logit_rules: the output's type");
-  if (out_pitch < z->classes || out_pitch > kMaxPitch) return fail(CREC_E_INVALID, "logit_rules: the output's pitch");
+  if (!fits_pitch(out_pitch, z->classes, z->rows)) return fail(CREC_E_INVALID, "logit_rules: the output's pitch");
   if (z->lines == 0 || z->rows == 0) return CREC_OK;
   if (!out || reinterpret_cast<uintptr_t>(out) % type_bytes(out_type)) return fail(CREC_E_INVALID, "logit_rules: the output");
   if (!output_fits(z, out, out_type, out_pitch)) return fail(CREC_E_INVALID, "logit_rules: the output overlaps the logits");
@@ -547,6 +560,7 @@ int crec_ctc_greedy_lines(const crec_line_logits* z, const crec_rules* rules, in
   if (const char* m = rules_fault(rules)) return fail(CREC_E_INVALID, m);
   if (z->lines == 0) return CREC_OK;
   if (!counts || (z->rows > 0 && (!ids || !starts || !probs))) return fail(CREC_E_INVALID, "ctc_greedy_lines: no output");
+  if (!aligned4({counts, ids, starts, probs})) return fail(CREC_E_INVALID, "ctc_greedy_lines: the outputs' alignment");
   OnDeviceOf on;
   if (const cudaError_t e = on.enter(counts); e != cudaSuccess) return fail.cuda(e, "ctc_greedy_lines: counts");
   LineParams p = line_params(z, rules);
@@ -581,6 +595,7 @@ int crec_candidates_lines(const crec_line_logits* z, const crec_rules* rules, in
     return fail(CREC_E_RANGE, "candidates_lines: topk is 0 to min(16, classes - 1)");
   if (z->lines == 0 || z->rows == 0) return CREC_OK;
   if (!blank || (topk > 0 && (!ids || !logp))) return fail(CREC_E_INVALID, "candidates_lines: no output");
+  if (!aligned4({ids, logp, blank})) return fail(CREC_E_INVALID, "candidates_lines: the outputs' alignment");
   OnDeviceOf on;
   if (const cudaError_t e = on.enter(z->logits); e != cudaSuccess) return fail.cuda(e, "candidates_lines: the logits");
   LineParams p = line_params(z, rules);
@@ -645,11 +660,12 @@ int crec_adapters_logits(crec_adapters* h, const void* x, int64_t x_pitch, int64
   if (!h) return fail(CREC_E_INVALID, "adapters_logits: no handle");
   if (!is_logits_type(type)) return fail(CREC_E_INVALID, "adapters_logits: the logits' type");
   if (rows < 0 || rows > kMaxRows || lines < 0) return fail(CREC_E_INVALID, "adapters_logits: rows or lines");
-  if (x_pitch < h->k || x_pitch > kMaxPitch || x_pitch % 8 || reinterpret_cast<uintptr_t>(x) % 16)
+  if (!fits_pitch(x_pitch, h->k, rows) || x_pitch % 8 || reinterpret_cast<uintptr_t>(x) % 16)
     return fail(CREC_E_INVALID, "adapters_logits: x 16-byte aligned, its pitch a multiple of 8 and at least K");
-  if (pitch < h->classes || pitch > kMaxPitch || reinterpret_cast<uintptr_t>(logits) % type_bytes(type))
+  if (!fits_pitch(pitch, h->classes, rows) || reinterpret_cast<uintptr_t>(logits) % type_bytes(type))
     return fail(CREC_E_INVALID, "adapters_logits: the logits' pitch or alignment");
   if (lines == 0 || rows == 0) return CREC_OK;
+  if (!aligned4({line_at, adapter})) return fail(CREC_E_INVALID, "adapters_logits: line_at's or adapter's alignment");
   if (!x || !line_at || !logits) return fail(CREC_E_INVALID, "adapters_logits: no x, line_at or logits");
   OnDeviceOf on;
   if (const cudaError_t e = on.to(h->device); e != cudaSuccess) return fail.cuda(e, "adapters_logits");

@@ -293,7 +293,7 @@ CREC_API int crec_head_sweep(int device, int precision, const void* model, size_
  * default stream) and not waited for; nothing is allocated and no scratch is shared, so calls may
  * overlap on different streams, be captured into CUDA graphs and be replayed.  The small structs
  * are read by the call itself.  No handle: a message for an error goes to error[0, error_size)
- * (may be null).  line_at ascends from 0 or more to at most `rows`; rows outside
+ * (may be null).  Arrays of 4-byte values are 4-byte aligned (CREC_E_INVALID).  line_at ascends from 0 or more to at most `rows`; rows outside
  * [line_at[0], line_at[lines]) are not written.  What is only known on the GPU cannot
  * be refused: a line_at that does not ascend gives unspecified results within the arrays.  No
  * counterpart in the reference, whose decoders know no rules. */
@@ -302,7 +302,7 @@ typedef struct crec_line_logits {
   int type;           /* CREC_FP32 or CREC_FP16 */
   int classes;        /* 1 to 65536 */
   int64_t pitch;      /* at least classes */
-  int64_t rows;       /* frames the array holds, at most 2^31 - 1 */
+  int64_t rows;       /* frames the array holds, at most 2^31 - 256 */
   int lines;
   const int32_t* line_at; /* [lines + 1] */
 } crec_line_logits;
@@ -384,7 +384,7 @@ CREC_API int crec_adapters_open(int device, const void* model, size_t model_byte
 /* Waits for the GPU and frees the handle (null: nothing). CREC_E_TIMEOUT if a launch's bounded wait ran out. */
 CREC_API int crec_adapters_close(crec_adapters* h);
 /* The lines' logits.  Device arrays: x float16 [rows][K], rows x_pitch elements apart (x 16-byte
- * aligned, x_pitch a multiple of 8), line_at [lines + 1] and adapter [lines] (null: the head
+ * aligned, x_pitch a multiple of 8; not in the logits), line_at [lines + 1] and adapter [lines] (null: the head
  * alone), logits of type `type` (CREC_FP32 or CREC_FP16), rows `pitch` elements apart.  Queued on
  * `stream`, nothing allocated, no scratch shared: calls may overlap, be captured and replayed.
  * Rows outside [line_at[0], line_at[lines]) are not written.  Every wait inside is bounded: after

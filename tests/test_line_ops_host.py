@@ -29,7 +29,8 @@ CALLS = [lambda z, r=None: native.logit_rules(z, r, 4096), lambda z, r=None: nat
 @pytest.mark.parametrize("call", CALLS)
 @pytest.mark.parametrize("wrong", [dict(type=0), dict(type=7), dict(classes=0), dict(classes=-3), dict(pitch=9), dict(pitch=1 << 41),
                                    dict(rows=-1), dict(rows=1 << 31), dict(lines=-1), dict(line_at=0), dict(logits=0),
-                                   dict(logits=66), dict(logits=65, type=native.FP16)])
+                                   dict(logits=66), dict(logits=65, type=native.FP16), dict(line_at=66),
+                                   dict(pitch=1 << 40, rows=1 << 30), dict(rows=(1 << 31) - 255)])
 def test_logits_that_are_refused(call, wrong):
     refused(native.E_INVALID, call, frames(**wrong))
 
@@ -37,7 +38,8 @@ def test_logits_that_are_refused(call, wrong):
 @pytest.mark.parametrize("call", CALLS)
 @pytest.mark.parametrize("wrong", [dict(history=64), dict(history_at=64), dict(repeat=64), dict(presence=64), dict(bias=64),
                                    dict(bias_of=64), dict(bias=64, biases=-1), dict(allowed=64), dict(set_of=64),
-                                   dict(allowed=64, sets=0)])
+                                   dict(allowed=64, sets=0), dict(history=66, history_at=64), dict(bias=65, biases=1),
+                                   dict(allowed=64, sets=1, set_of=62)])
 def test_rules_that_are_refused(call, wrong):
     refused(native.E_INVALID, call, frames(), native.Rules(**wrong))
 
@@ -70,6 +72,8 @@ def test_outputs_that_are_missing():
     for i in range(4):
         out = [0 if j == i else 64 for j in range(4)]
         refused(native.E_INVALID, native.ctc_greedy_lines, frames(), None, *out)
+    refused(native.E_INVALID, native.ctc_greedy_lines, frames(), None, 64, 64, 66, 64)
+    refused(native.E_INVALID, native.candidates_lines, frames(), None, 3, 64, 65, 64)
     for out in ((0, 64, 64), (64, 0, 64), (64, 64, 0)):
         refused(native.E_INVALID, native.candidates_lines, frames(), None, 3, *out)
 
