@@ -205,9 +205,9 @@ cudaError_t decode(LineParams& p, cudaStream_t s) {
 }
 
 // Long rows where lines are long too: a block sets a line's rules for 8 or 16 warps, so from 16 frames a
-// line on average (fewer leave warps idle and pay the rules more often than a team does: 140 us against
-// 105 at 8 and 30 frames a line of 12,000 classes), and from 2,048 classes (1,500: 227 us against a team's
-// 204; 2,900: 192 against 209; 12,000: 85 against 127).
+// line on average (candidates of 4,096 x 12,000 float16: 118 us against a team's 134 at 16 frames a line,
+// 161 against 140 at 8), and from 2,048 classes (75 frames a line, as many logits: 1,504 classes 126 us
+// against 124, 2,900 132 against 140, 12,000 85 against 128).
 constexpr int kLongLines = 16, kLongClasses = 2048;
 
 template <int kOp, typename T, int V>
@@ -219,7 +219,8 @@ cudaError_t decode_long(LineParams& p, cudaStream_t s) {
   const int chunks = (p.classes + L::kChunk - 1) / L::kChunk;
   const size_t rules = sizeof(TeamRow) + kLongEntries * 10 + static_cast<size_t>(chunks) * L::kChunk * 4;
   // Two blocks of 8 warps an SM, one at work while the other sets rules, or one of 16, whose rules serve
-  // twice the rows: the first up to 8,192 classes (12,000: 104 us against 85; 2,900: 192 against 209).
+  // twice the rows: the first up to 8,192 classes (12,000: 104 us against 85; 6,000 alike; 2,900: 192
+  // against 209 before rows of any address were copied in 16-byte pieces).
   p.warps = p.classes <= 8192 ? kMaxTeam / 2 : kMaxTeam;
   const int blocks = sms * (kMaxTeam / p.warps);
   p.team_rows = (p.rows + blocks - 1) / blocks;
