@@ -411,27 +411,32 @@ void plan_adapters(const crec_adapters* h, AdapterParams* p) {
   p->boxes = p->width >= 16 && room - kBoxBytes >= 3 * 8192;
   if (p->boxes) room -= kBoxBytes;
   // Of tiles of 128 frames or fewer, chunks of kAdapterChunk classes or fewer and a tile's chunks in one
-  // part or as many as reach every SM, the cheapest: rounds of SMs times what a part takes, in 0.1 us as
-  // measured (K = 256, 160 classes a chunk): 4 us for its frames and h, 0.4 us a block of 64 channels a
-  // chunk, 0.5 us an adapter a chunk, and not less than its logits take at an SM's share of HBM.  Fewer
-  // frames a tile mean fewer adapters in it, whose MMAs come one after another.
+  // part, two, or as many as fill the SMs once, twice or three times, the cheapest: rounds of SMs times
+  // what a part takes, in 0.1 us as measured (K = 256, 160 classes a chunk): 4 us for its frames and h,
+  // 0.4 us a block of 64 channels a chunk, 0.5 us an adapter a chunk, and not less than its logits take
+  // at an SM's share of HBM.  Fewer frames a tile mean fewer adapters in it, whose MMAs come one after
+  // another.
   double least = 0;
   for (int rows = 128; rows >= 16; rows /= 2) {
     const int tiles = (p->rows + rows - 1) / rows;
     const double lines = std::min<double>(rows, 1.0 + static_cast<double>(p->lines) * rows / p->rows);  // that a tile meets
     const double slots = p->adapter ? std::min<double>(lines, h->adapters) : 0.0;
+    int last_n = 0;
     for (const int wide : {224, 160, 96, 64, 32}) {
       const int most = std::max(unit, wide / unit * unit), chunks = (h->classes + most - 1) / most;
       const int n = ((h->classes + chunks - 1) / chunks + unit - 1) / unit * unit;
       const int stage = std::max(n * 128, 8192), stages = std::min(kAdapterStages, room / stage);
-      if (stages < 2 || (stages < 3 && n > unit)) continue;
+      if (stages < 2 || (stages < 3 && n > unit) || n == last_n) continue;
+      last_n = n;
       const double chunk = std::max(p->nkb * (2.0 + n / 80.0) + slots * (2.0 + n / 60.0) * ((p->rank + 15) / 16),
                                     static_cast<double>(rows) * n * (p->half ? 2 : 4) / 4300.0);
-      const int most_parts = std::min(chunks, std::max(1, h->sms / tiles));
-      for (const int s : {1, 2, most_parts}) {
-        if (s > chunks) continue;
+      int before = 0;
+      for (const int fill : {1, 2, h->sms / tiles, 2 * h->sms / tiles, 3 * h->sms / tiles}) {
+        const int s = std::min(fill, chunks);
+        if (s <= before) continue;
+        before = s;
         const int per = (chunks + s - 1) / s, parts = (chunks + per - 1) / per;
-        const long long rounds = (static_cast<long long>(tiles) * parts + h->sms - 1) / h->sms;
+        const int rounds = (tiles * parts + h->sms - 1) / h->sms;  // (2 parts of 2^27 tiles at most)
         const double cost = rounds * (40.0 + slots * p->nkb * 0.5 + per * chunk);
         if (least != 0 && cost >= least) continue;
         least = cost;
