@@ -597,7 +597,7 @@ int crec_candidates_lines(const crec_line_logits* z, const crec_rules* rules, in
   const Errors fail{error, error_size};
   if (const char* m = lines_fault(z)) return fail(CREC_E_INVALID, m);
   if (const char* m = rules_fault(rules)) return fail(CREC_E_INVALID, m);
-  if (topk < 0 || topk > std::min(16, z->classes - 1))
+  if (topk < 0 || topk > std::min(kMaxTop, z->classes - 1))
     return fail(CREC_E_RANGE, "candidates_lines: topk is 0 to min(16, classes - 1)");
   if (z->lines == 0 || z->rows == 0) return CREC_OK;
   if (!blank || (topk > 0 && (!ids || !logp))) return fail(CREC_E_INVALID, "candidates_lines: no output");

@@ -48,7 +48,7 @@ struct LineParams {
   int bias_wide;  // the bias tables' rows may be read 16 bytes at a time
 };
 
-constexpr int kOpRules = 0, kOpGreedy = 1, kOpCandidates = 2;
+constexpr int kOpGreedy = 1, kOpCandidates = 2;
 
 // One line's rules.
 struct LineRule {
