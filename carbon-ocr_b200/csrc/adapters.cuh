@@ -9,7 +9,7 @@
 // moved, and the cost goes with the distinct adapters of a tile, not its lines.  First h: the A rows
 // of as many slots as 64 columns of TMEM hold as one B operand, each such group's product kept for its
 // slots' frames only, so that all groups share the columns; a frame reads its own slot's.
-// Four warps scale it and put it back as an A operand, as two tf32 words whose sum holds 22 bits (h
+// Four warps scale it and put it back as an A operand, as two tf32 words whose sum is within 2^-23 of it (h
 // rounded to float16 once would cost the logits 2^-11 of the adapter's part, and its range; B's
 // float16 values are tf32 values exactly).  Then each slot's B rows over each chunk's accumulators.
 #pragma once
@@ -554,8 +554,9 @@ __global__ void __launch_bounds__(kAdapterThreads, 1) adapter_head_kernel(const 
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const float v = __fmul_rn(__uint_as_float(r[j + i]), scale);
-            hi[i] = __float_as_uint(v) & 0xffffe000u;  // tf32: 10 bits of the fraction
-            lo[i] = __float_as_uint(__fsub_rn(v, __uint_as_float(hi[i])));
+            // tf32 holds 10 bits of the fraction (the MMA drops the rest): each word rounded to them
+            hi[i] = (__float_as_uint(v) + 0x1000u) & 0xffffe000u;
+            lo[i] = (__float_as_uint(__fsub_rn(v, __uint_as_float(hi[i]))) + 0x1000u) & 0xffffe000u;
           }
           // 16 bytes of row t: in rows of rank_row bytes, swizzled as the MMA reads them
           const int k = j0 + j, block = k / 32, piece = (k % 32) / 4;
