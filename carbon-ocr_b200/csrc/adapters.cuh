@@ -12,6 +12,8 @@
 // Four warps scale it and put it back as an A operand, as two tf32 words whose sum is within 2^-23 of it (h
 // rounded to float16 once would cost the logits 2^-11 of the adapter's part, and its range; B's
 // float16 values are tf32 values exactly).  Then each slot's B rows over each chunk's accumulators.
+// Ranks are padded to the handle's with rows of zeros; h past an adapter's own rank is written as 0,
+// since a frame's infinity times those zeros is NaN.
 #pragma once
 
 #include <cuda.h>
@@ -43,6 +45,7 @@ struct AdapterParams {
   int adapters;
   const float* bias;   // [classes], then 256 zeros
   const float* scale;  // [adapters]
+  const int32_t* own;  // [adapters] ranks before they are padded
   void* z;
   long long pitch;
   int half;
@@ -69,7 +72,8 @@ struct TileSlots {
   uint4 rows[128];  // each slot's frames, a bit each
   uint4 group[128];  // and each group's
   int id[128];      // and its adapter
-  int slot[128];    // each frame's slot, -1 none, -2 not a line's frame
+  int16_t slot[128];  // each frame's slot, -1 none, -2 not a line's frame
+  int16_t own[128];   // and its adapter's own rank
   float scale[128];
 };
 
@@ -172,9 +176,21 @@ __device__ __forceinline__ void find_slots(const AdapterParams& p, AdapterShared
     atomicOr(reinterpret_cast<uint32_t*>(&tile.rows[slot]) + q, 1u << lane);
     atomicOr(reinterpret_cast<uint32_t*>(&tile.group[slot / (64 / p.r16)]) + q, 1u << lane);
   }
-  tile.slot[t] = slot;
+  tile.slot[t] = static_cast<int16_t>(slot);
+  tile.own[t] = static_cast<int16_t>(id >= 0 ? p.own[id] : 0);
   tile.scale[t] = id >= 0 ? p.scale[id] : 0.0f;
   if (t == 0) tile.n = all;
+}
+
+// v as two tf32 words (10 bits of the fraction, the MMA drops the rest), each rounded to them: hi + lo is
+// within 2^-23 of v.  Rounding adds half a unit to the bits, so three kinds are told apart: finite
+// values that it would carry to infinity are cut instead (lo takes what is cut off), an infinity is hi
+// alone, and a NaN is one that keeps its kind without its low bits (the carry would make it 0).
+__device__ __forceinline__ void split_tf32(float v, uint32_t& hi, uint32_t& lo) {
+  constexpr uint32_t kKept = 0xffffe000u, kInf = 0x7f800000u, kCarries = 0x7f7ff000u;
+  const uint32_t b = __float_as_uint(v), size = b & 0x7fffffffu;
+  hi = size > kInf ? 0x7fffe000u : size >= kCarries ? b & kKept : (b + 0x1000u) & kKept;
+  lo = size >= kInf ? 0u : (__float_as_uint(__fsub_rn(v, __uint_as_float(hi))) + 0x1000u) & kKept;
 }
 
 // 16 logits of one frame (c the first's class) from their accumulators.
@@ -530,6 +546,7 @@ __global__ void __launch_bounds__(kAdapterThreads, 1) adapter_head_kernel(const 
         continue;
       }
       const float scale = tile.scale[t];
+      const int own = tile.own[t];
       const int place = max(tile.slot[t], 0) % per_group * p.r16;  // this frame's columns of h
       ok = mbar_wait_warp(&s.h_full, hits & 1, p.err, kErrTimeoutFull, p.wait_ns) &&
            mbar_wait_warp(&s.h2_empty, (hits & 1) ^ 1, p.err, kErrTimeoutEmpty, p.wait_ns);
@@ -552,12 +569,8 @@ __global__ void __launch_bounds__(kAdapterThreads, 1) adapter_head_kernel(const 
           if (j0 + j >= p.rank) break;
           uint32_t hi[4], lo[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float v = __fmul_rn(__uint_as_float(r[j + i]), scale);
-            // tf32 holds 10 bits of the fraction (the MMA drops the rest): each word rounded to them
-            hi[i] = (__float_as_uint(v) + 0x1000u) & 0xffffe000u;
-            lo[i] = (__float_as_uint(__fsub_rn(v, __uint_as_float(hi[i]))) + 0x1000u) & 0xffffe000u;
-          }
+          for (int i = 0; i < 4; ++i)
+            split_tf32(j0 + j + i < own ? __fmul_rn(__uint_as_float(r[j + i]), scale) : 0.0f, hi[i], lo[i]);
           // 16 bytes of row t: in rows of rank_row bytes, swizzled as the MMA reads them
           const int k = j0 + j, block = k / 32, piece = (k % 32) / 4;
           const int swz = piece ^ ((t * p.rank_row >> 7) & (p.rank_row / 16 - 1));

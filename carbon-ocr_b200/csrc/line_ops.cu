@@ -311,6 +311,7 @@ struct crec_adapters {
   __half* a = nullptr;   // [adapters][r16][k]
   float* b = nullptr;    // [adapters][classes][rank]
   float* scale = nullptr;
+  int32_t* own = nullptr;  // [adapters] ranks before they are padded
   std::atomic<bool> inject{false};  // the next launch's waits run out (crec_adapters_inject)
   int* err = nullptr;  // pinned, written by a launch whose bounded wait ran out
 };
@@ -458,7 +459,7 @@ void free_adapters(crec_adapters* h) {
   OnDeviceOf on;
   if (on.to(h->device) == cudaSuccess) {
     for (void* p : {static_cast<void*>(h->w), static_cast<void*>(h->bias), static_cast<void*>(h->a),
-                    static_cast<void*>(h->b), static_cast<void*>(h->scale)})
+                    static_cast<void*>(h->b), static_cast<void*>(h->scale), static_cast<void*>(h->own)})
       cudaFree(p);
     cudaFreeHost(h->err);
   }
@@ -525,6 +526,7 @@ int open_adapters(int device, const void* model, size_t model_bytes, int n, cons
   if (e == cudaSuccess) e = to_device(&h->a, pa.data(), na);
   if (e == cudaSuccess) e = to_device(&h->b, pb.data(), nb);
   if (e == cudaSuccess) e = to_device(&h->scale, scales, static_cast<size_t>(n));
+  if (e == cudaSuccess) e = to_device(&h->own, ranks, static_cast<size_t>(n));
   if (e == cudaSuccess) e = cudaHostAlloc(reinterpret_cast<void**>(&h->err), sizeof(int), cudaHostAllocMapped);
   if (e == cudaSuccess) *h->err = 0;
   if (e == cudaSuccess)
@@ -685,6 +687,7 @@ int crec_adapters_logits(crec_adapters* h, const void* x, int64_t x_pitch, int64
   p.adapters = h->adapters;
   p.bias = h->bias;
   p.scale = h->scale;
+  p.own = h->own;
   p.z = logits;
   p.pitch = pitch;
   p.half = type == CREC_FP16;

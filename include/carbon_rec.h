@@ -367,7 +367,9 @@ CREC_API int crec_candidates_lines(const crec_line_logits* z, const crec_rules* 
  * beside it, one a line: frame f of line i gets
  *   z[f][c] = sum_k x[f][k] W[c][k] + b[c] + scale_a * sum_j (sum_k x[f][k] A_a[j][k]) B_a[c][j]
  * with a = adapter[i] (outside [0, adapters): the head alone).  float16 features, weights and
- * adapters, float32 sums (the adapters' inner sums too). */
+ * adapters, float32 sums (the adapters' inner sums too).  NaN and infinities show in the logits that
+ * the formula has them in and in no others; an infinity in B may give NaN where the formula has an
+ * infinity. */
 typedef struct crec_adapters crec_adapters;
 
 /* The channels and classes of the head of `model`: a float recognizer's blob, or
