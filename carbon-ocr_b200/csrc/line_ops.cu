@@ -150,10 +150,15 @@ cudaError_t sm_count(int* out) {
   return cudaSuccess;
 }
 
+// A block's largest dynamic shared memory is an attribute of the kernel, on its device, for every thread
+// of the program: each call sets the same value, the most that any of these launches may take (227 KB
+// less 1 KB for static variables), so that none lowers it between another's setting and launch.
+constexpr int kMostShared = 232448 - 1024;
+
 template <typename K>
 cudaError_t launch_on(K* k, const LineParams& p, long long blocks, int threads, size_t smem, cudaStream_t s) {
   if (smem > 48 << 10) {
-    const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostShared);
     if (e != cudaSuccess) return e;
   }
   k<<<static_cast<unsigned>(blocks), threads, smem, s>>>(p);
