@@ -235,6 +235,12 @@ __device__ __forceinline__ float warp_max_nan(float v) {
   asm("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
   return m;
 }
+// The same of two.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float m;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+  return m;
+}
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
   for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -1319,7 +1325,8 @@ __global__ void __launch_bounds__(32 * kMaxTeam) wide_rows_kernel(const __grid_c
 // Greedy CTC's second half, a warp a line, in place: ids and probs hold each frame's class and
 // probability; the characters go to the front of the line's places (never past the frames already
 // read), the rest is filled.  The frames of four steps are read at once: their latency, not their
-// bytes, is what this kernel takes.
+// bytes, is what this kernel takes.  A NaN among a character's frames stays its maximum, whatever the
+// order that the frames are joined in.
 __global__ void __launch_bounds__(128) collapse_lines_kernel(const __grid_constant__ LineParams p) {
   const int i = blockIdx.x * 4 + threadIdx.x / 32, lane = threadIdx.x % 32;
   int first = 0, end = 0;
@@ -1358,9 +1365,9 @@ __global__ void __launch_bounds__(128) collapse_lines_kernel(const __grid_consta
         for (int o = 1; o < 32; o <<= 1) {
           const float up = __shfl_up_sync(0xffffffffu, pr, o);
           const int uid = __shfl_up_sync(0xffffffffu, id, o);
-          if (lane >= o && uid == id && (mine & ~(upto >> o)) == 0) pr = up > pr ? up : pr;
+          if (lane >= o && uid == id && (mine & ~(upto >> o)) == 0) pr = max_nan(up, pr);
         }
-        if (id != 0 && id == before && mine == 0) pr = carry > pr ? carry : pr;
+        if (id != 0 && id == before && mine == 0) pr = max_nan(carry, pr);
       }
       const int after = __shfl_down_sync(0xffffffffu, id, 1);
       const bool last = id != 0 && (lane == 31 || after != id);

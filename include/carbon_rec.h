@@ -348,7 +348,7 @@ CREC_API int crec_logit_rules(const crec_line_logits* z, const crec_rules* rules
  * start -1, probability 0.  ids, starts and probs hold `rows` entries.  The ids, counts and
  * starts are those of the definition exactly; the probabilities' sums are taken in float32 in
  * another order than crec_ctc_greedy's.  A NaN that is allowed wins no frame and makes its
- * frame's probability NaN, as does an allowed +inf. */
+ * frame's probability NaN, as does an allowed +inf; a character with such a frame has probability NaN. */
 CREC_API int crec_ctc_greedy_lines(const crec_line_logits* z, const crec_rules* rules, int32_t* counts, int32_t* ids,
                                    int32_t* starts, float* probs, void* stream, char* error, size_t error_size);
 
