@@ -750,7 +750,7 @@ __device__ __noinline__ void slow_row(const LineParams& p, int r, LineRule l, Te
     if constexpr (kOp == kOpGreedy) {
       arg = __reduce_min_sync(0xffffffffu, lane < warps ? t.arg[0][lane] : 0xffffffffu);
       if (lane == 0) {
-        p.ids[r] = static_cast<int32_t>(arg);
+        p.ids[r] = some ? static_cast<int32_t>(arg) : 0;  // nothing left but a NaN that the blank holds: blank
         p.probs[r] = __fdiv_rn(from.term(best), sum);
       }
     } else {
@@ -911,7 +911,7 @@ __global__ void __launch_bounds__(32 * kMaxTeam, 1) line_rows_kernel(const __gri
           arg = __reduce_min_sync(0xffffffffu, lane < warps ? t.arg[parity][lane] : 0xffffffffu);
         }
         if (lane == 0) {
-          p.ids[r] = static_cast<int32_t>(arg);
+          p.ids[r] = static_cast<int32_t>(arg);  // (0 where nothing is left: the blank's own place holds -inf)
           p.probs[r] = __fdiv_rn(from.term(best), sum + from.term(blank));
         }
       }
@@ -1282,7 +1282,7 @@ __global__ void __launch_bounds__(32 * kMaxTeam, 1) long_rows_kernel(const __gri
       sum += from.term(blank);
       if constexpr (kOp == kOpGreedy) {
         if (lane == 0) {
-          p.ids[row] = static_cast<int32_t>(arg);
+          p.ids[row] = some ? static_cast<int32_t>(arg) : 0;  // as slow_row
           p.probs[row] = __fdiv_rn(from.term(all), sum);
         }
       } else {

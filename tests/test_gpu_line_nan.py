@@ -39,3 +39,36 @@ def test_a_nan_shows_in_its_characters_probability(classes):
         else:
             assert abs(probs[a] - wpr[0]) <= ROOM
         assert abs(probs[a + 1] - wpr[1]) <= ROOM
+
+
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("classes", CLASSES)
+@pytest.mark.parametrize("named", [0, 400])
+def test_a_nan_with_nothing_left_beside_it(classes, half, named):
+    """Frames whose classes are NaN or nothing: they are blanks, and no candidate is left.  `named`: so many
+    classes in the lines' histories (more than 256 go another way)."""
+    rng = np.random.default_rng(classes + half)
+    lines = 36 if classes <= 1500 else 3  # (enough rows for a warp to take its rows alone)
+    at = line_places(rng, [40] * lines)
+    z = logits_of(rng, at[-1], classes, half)
+    z[:, 0] = -20
+    nothing = [0, 3, 4, 39, 45, 79, 80, 90, 119]
+    for i, t in enumerate(nothing):
+        z[t] = np.nan if i % 3 == 0 else -np.inf
+        z[t, 0] = np.nan
+    rules = None
+    if named:
+        ids = [rng.permutation(classes)[:named] for _ in range(lines)]
+        rules = {"history": np.concatenate(ids).astype(np.int32), "repeat": np.full(lines, 1.25, np.float32),
+                 "history_at": np.concatenate([[0], np.cumsum([len(i) for i in ids])]).astype(np.int32)}
+    c = Case(z, at, rules)
+    c.want[nothing, 1:] = -np.inf  # (a NaN wins nothing)
+    c.want[nothing, 0] = 0
+    want = R.greedy(c.want, at)
+    counts, ids, starts, _ = (x.cpu().numpy() for x in c.greedy())
+    for i, (wid, wst, _) in enumerate(want):
+        assert counts[i] == len(wid)
+        assert ids[at[i]:at[i] + counts[i]].tolist() == wid and starts[at[i]:at[i] + counts[i]].tolist() == wst
+    ids, logp, blank = (x.cpu().numpy() for x in c.candidates(3))
+    assert (ids[nothing] == -1).all() and np.isneginf(logp[nothing]).all() and np.isnan(blank[nothing]).all()
+    assert (np.delete(ids, nothing, 0) > 0).all() and np.isfinite(np.delete(blank, nothing, 0)).all()
