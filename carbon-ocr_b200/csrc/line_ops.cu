@@ -71,6 +71,7 @@ class OnDeviceOf {
 size_t type_bytes(int type) { return type == CREC_FP16 ? 2 : 4; }
 bool is_logits_type(int type) { return type == CREC_FP32 || type == CREC_FP16; }
 constexpr int64_t kMaxRows = 0x7fffff00;  // a tile past them still counts in 32 bits
+constexpr int kMaxLines = 0x7fffff00;     // and a step of the lines' search
 
 // Whether an array of `rows` rows has such a pitch (its bytes far within 64 bits).
 bool fits_pitch(int64_t pitch, int64_t least, int64_t rows) {
@@ -88,7 +89,7 @@ const char* lines_fault(const crec_line_logits* z) {
   if (!z) return "no logits";
   if (!is_logits_type(z->type)) return "the logits' type";
   if (z->classes < 1 || z->classes > kMaxClasses) return "classes";
-  if (z->rows < 0 || z->rows > kMaxRows || z->lines < 0) return "rows or lines";
+  if (z->rows < 0 || z->rows > kMaxRows || z->lines < 0 || z->lines > kMaxLines) return "rows or lines";
   if (!fits_pitch(z->pitch, z->classes, z->rows)) return "pitch";
   if (!aligned4({z->line_at})) return "line_at's alignment";
   if (z->lines > 0 && !z->line_at) return "no line_at";
@@ -227,9 +228,9 @@ cudaError_t decode_long(LineParams& p, cudaStream_t s) {
   // twice the rows: the first up to 8,192 classes (12,000: 104 us against 85; 6,000 alike; 2,900: 192
   // against 209 before rows of any address were copied in 16-byte pieces).
   p.warps = p.classes <= 8192 ? kMaxTeam / 2 : kMaxTeam;
-  const int blocks = sms * (kMaxTeam / p.warps);
-  p.team_rows = (p.rows + blocks - 1) / blocks;
-  return launch_on(long_rows_kernel<kOp, T, V>, p, (p.rows + p.team_rows - 1) / p.team_rows, 32 * p.warps, rules + p.warps * L::kWarp, s);
+  const long long blocks = sms * (kMaxTeam / p.warps);
+  p.team_rows = static_cast<int>((p.rows + blocks - 1) / blocks);
+  return launch_on(long_rows_kernel<kOp, T, V>, p, (static_cast<long long>(p.rows) + p.team_rows - 1) / p.team_rows, 32 * p.warps, rules + p.warps * L::kWarp, s);
 }
 
 template <int kOp, typename T>
@@ -246,7 +247,7 @@ cudaError_t write_rows(LineParams& p, int sms, cudaStream_t s) {
   const size_t smem = static_cast<size_t>(kWarps) * Row::kShared;
   const long long resident = blocks_an_sm(smem, kWarps, 32) * static_cast<long long>(kWarps) * sms;
   p.team_rows = static_cast<int>(std::max(1ll, (static_cast<long long>(p.rows) * p.chunks + resident - 1) / resident));
-  const long long units = (p.rows + p.team_rows - 1) / p.team_rows * static_cast<long long>(p.chunks);
+  const long long units = (static_cast<long long>(p.rows) + p.team_rows - 1) / p.team_rows * p.chunks;
   return launch_on(logit_rules_kernel<T, O, V, NV>, p, (units + kWarps - 1) / kWarps, kRulesThreads, smem, s);
 }
 
@@ -672,7 +673,7 @@ int crec_adapters_logits(crec_adapters* h, const void* x, int64_t x_pitch, int64
   const Errors fail{error, error_size};
   if (!h) return fail(CREC_E_INVALID, "adapters_logits: no handle");
   if (!is_logits_type(type)) return fail(CREC_E_INVALID, "adapters_logits: the logits' type");
-  if (rows < 0 || rows > kMaxRows || lines < 0) return fail(CREC_E_INVALID, "adapters_logits: rows or lines");
+  if (rows < 0 || rows > kMaxRows || lines < 0 || lines > kMaxLines) return fail(CREC_E_INVALID, "adapters_logits: rows or lines");
   if (!fits_pitch(x_pitch, h->k, rows) || x_pitch % 8 || reinterpret_cast<uintptr_t>(x) % 16)
     return fail(CREC_E_INVALID, "adapters_logits: x 16-byte aligned, its pitch a multiple of 8 and at least K");
   if (!fits_pitch(pitch, h->classes, rows) || reinterpret_cast<uintptr_t>(logits) % type_bytes(type))

@@ -303,7 +303,7 @@ typedef struct crec_line_logits {
   int classes;        /* 1 to 65536 */
   int64_t pitch;      /* at least classes */
   int64_t rows;       /* frames the array holds, at most 2^31 - 256 */
-  int lines;
+  int lines;              /* at most 2^31 - 256 */
   const int32_t* line_at; /* [lines + 1] */
 } crec_line_logits;
 
@@ -386,7 +386,7 @@ CREC_API int crec_adapters_open(int device, const void* model, size_t model_byte
 /* Waits for the GPU and frees the handle (null: nothing). CREC_E_TIMEOUT if a launch's bounded wait ran out. */
 CREC_API int crec_adapters_close(crec_adapters* h);
 /* The lines' logits.  Device arrays: x float16 [rows][K], rows x_pitch elements apart (x 16-byte
- * aligned, x_pitch a multiple of 8; not in the logits), line_at [lines + 1] and adapter [lines] (null: the head
+ * aligned, x_pitch a multiple of 8; not in the logits; rows and lines as crec_line_logits'), line_at [lines + 1] and adapter [lines] (null: the head
  * alone), logits of type `type` (CREC_FP32 or CREC_FP16), rows `pitch` elements apart.  Queued on
  * `stream`, nothing allocated, no scratch shared: calls may overlap, be captured and replayed.
  * Rows outside [line_at[0], line_at[lines]) are not written.  Every wait inside is bounded: after
