@@ -225,9 +225,11 @@ cudaError_t decode_long(LineParams& p, cudaStream_t s) {
   const int chunks = (p.classes + L::kChunk - 1) / L::kChunk;
   const size_t rules = sizeof(TeamRow) + kLongEntries * 10 + static_cast<size_t>(chunks) * L::kChunk * 4;
   // Two blocks of 8 warps an SM, one at work while the other sets rules, or one of 16, whose rules serve
-  // twice the rows: the first up to 8,192 classes (12,000: 104 us against 85; 6,000 alike; 2,900: 192
-  // against 209 before rows of any address were copied in 16-byte pieces).
-  p.warps = p.classes <= 8192 ? kMaxTeam / 2 : kMaxTeam;
+  // twice the rows: the first up to 5,000 classes.  Candidates (k = 16, 75 frames a line, 98 MB), 8 against
+  // 16 warps: float16 2,904 classes 100 us against 105, 4,096 89 against 94, 6,000 93 against 89, 12,000 107
+  // against 89; float32 2,904 73 against 78, 4,096 73 against 80, 6,000 76 against 68, 12,000 95 against 78;
+  // rows of any address (float16) 2,901 134 against 141, 6,001 123 against 123, 9,001 134 against 123.
+  p.warps = p.classes <= 5000 ? kMaxTeam / 2 : kMaxTeam;
   const long long blocks = sms * (kMaxTeam / p.warps);
   p.team_rows = static_cast<int>((p.rows + blocks - 1) / blocks);
   return launch_on(long_rows_kernel<kOp, T, V>, p, (static_cast<long long>(p.rows) + p.team_rows - 1) / p.team_rows, 32 * p.warps, rules + p.warps * L::kWarp, s);
