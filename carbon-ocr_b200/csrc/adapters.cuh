@@ -51,6 +51,7 @@ struct AdapterParams {
   int half;
   int width;  // bytes that a row of z may be written at once: 32, 16, or an element's
   int boxes;  // z's rows are 16-byte aligned and shared memory has room: whole boxes go out by TMA
+  int clipped;  // a row's classes are whole 16-byte pieces (a TMA store ends at a piece, not at an element): so do clipped ones
   // tiles
   int tile_rows;                      // frames a tile takes of the 128 rows of an MMA
   int n, chunks, splits, chunks_per;  // classes a chunk (a multiple of 128 bytes of z's); a tile's chunks, in `splits` parts
@@ -611,7 +612,15 @@ __global__ void __launch_bounds__(kAdapterThreads, 1) adapter_head_kernel(const 
         if (whole) {  // boxes, the two halves in turn
           const int step = p.half ? 64 : 32;
           for (int k = half * step; k < p.n && c * p.n + k < p.classes; k += 2 * step) {
-            if (p.half) store_box<true>(p, box, taddr + k, lane, t * p.tile_rows + quarter * 32, c * p.n + k, bias + k);
+            if (!p.clipped && c * p.n + k + step > p.classes) {  // what follows a row's classes is not ours to write
+              for (int g = k; g < k + step && c * p.n + g < p.classes; g += 16) {
+                uint32_t v[16];
+                tmem_ld16(taddr + g, v);
+                tmem_wait_ld();
+                tmem_pin(v);
+                if (mine) store_logits(p, r, c * p.n + g, v, bias + g);
+              }
+            } else if (p.half) store_box<true>(p, box, taddr + k, lane, t * p.tile_rows + quarter * 32, c * p.n + k, bias + k);
             else store_box<false>(p, box, taddr + k, lane, t * p.tile_rows + quarter * 32, c * p.n + k, bias + k);
           }
         } else {

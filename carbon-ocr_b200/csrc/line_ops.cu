@@ -419,6 +419,7 @@ void plan_adapters(const crec_adapters* h, AdapterParams* p) {
   const int unit = p->half ? 64 : 32;  // a box's classes
   p->boxes = p->width >= 16 && room - kBoxBytes >= 3 * 8192;
   if (p->boxes) room -= kBoxBytes;
+  p->clipped = h->classes * (p->half ? 2ll : 4ll) % 16 == 0;
   // Of tiles of 128 frames or fewer, chunks of kAdapterChunk classes or fewer and a tile's chunks in one
   // part, two, or as many as fill the SMs once, twice or three times, the cheapest: rounds of SMs times
   // what a part takes, in 0.1 us as measured (K = 256, 160 classes a chunk): 4 us for its frames and h,
