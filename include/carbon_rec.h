@@ -199,7 +199,10 @@ CREC_API int crec_candidates(crec_handle* h, const int32_t* rows, int n, int top
  * for a head of the caller's own beside it (crec_adapters_logits): the lines' frames end to end, frame
  * f's channels at x + f * pitch, float16 on this handle's GPU (INT8: the codes' values, rounded),
  * line j's frames [line_at[j], line_at[j + 1]) (line_at [n + 1], host).  capacity: the frames x holds;
- * pitch in elements, at least the head's channels.  Waited for.  No counterpart in the reference. */
+ * pitch in elements, at least the head's channels.  A call of more lines or columns than one device
+ * run holds keeps its last run's lines only: others are refused (CREC_E_RANGE), so recognise no more
+ * than a run at a time where all lines are wanted.  Waited for on the host; line_at is the host's, to
+ * be copied to the GPU for the calls below.  No counterpart in the reference. */
 CREC_API int crec_head_input(crec_handle* h, const int32_t* rows, int n, int32_t* line_at, void* x, int64_t pitch,
                              int64_t capacity);
 
@@ -379,7 +382,10 @@ CREC_API int crec_blob_head(const void* model, size_t model_bytes, int* k, int* 
 /* The head of `model` (as crec_blob_head reads it, its weights rounded to float16) on GPU `device` with n adapters (0 or more): host arrays, ranks[i] the rank of adapter
  * i (1..64), a its A matrices [ranks[i]][K] one after another, b its B matrices [classes][ranks[i]]
  * one after another (float16 bits), scales [n].  K a multiple of 8, at most 512.  The arrays are
- * copied.  Synchronous; the handle is not changed by the calls that use it. */
+ * copied, every adapter padded to the largest rank among them (to 8, 16, 32 or 64): one of rank 64
+ * makes each of the others cost as much, so ranks far apart are better in handles of their own.
+ * Another set of adapters is another handle.  Synchronous; the handle is not changed by the calls
+ * that use it. */
 CREC_API int crec_adapters_open(int device, const void* model, size_t model_bytes, int n, const int32_t* ranks,
                                 const void* a, const void* b, const float* scales, crec_adapters** out, char* error,
                                 size_t error_size);
