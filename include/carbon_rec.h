@@ -201,8 +201,9 @@ CREC_API int crec_candidates(crec_handle* h, const int32_t* rows, int n, int top
  * line j's frames [line_at[j], line_at[j + 1]) (line_at [n + 1], host).  capacity: the frames x holds;
  * pitch in elements, at least the head's channels.  A call of more lines or columns than one device
  * run holds keeps its last run's lines only: others are refused (CREC_E_RANGE), so recognise no more
- * than a run at a time where all lines are wanted.  Waited for on the host; line_at is the host's, to
- * be copied to the GPU for the calls below.  No counterpart in the reference. */
+ * than a run at a time where all lines are wanted.  Waited for on the host, on this handle's stream:
+ * what other streams still do with x (an earlier call's logits from it) has to be done before.
+ * line_at is the host's, to be copied to the GPU for the calls below.  No counterpart in the reference. */
 CREC_API int crec_head_input(crec_handle* h, const int32_t* rows, int n, int32_t* line_at, void* x, int64_t pitch,
                              int64_t capacity);
 
